@@ -296,6 +296,102 @@ int qora_hip_attn_prefill(qora_hip_ctx* ctx, const float* q, const void* kc, con
  * written to a device int32. */
 int qora_hip_argmax(qora_hip_ctx* ctx, const float* logits, uint64_t n, int32_t* out_device, void* stream);
 
+/* ---- many requests at once -----------------------------------------------
+ * No counterpart in the reference, which decodes one request. A server keeps
+ * every request's keys and values in pages of one pool per layer and runs a
+ * batch of rows of many requests through the same weights: qora_hip_gemm_lora
+ * for the projections, qora_hip_paged_append, qora_hip_paged_attn_run. All of
+ * them can be captured into graphs: a batch's arrays are read on the device
+ * when the work runs, so a replay takes what they then hold. */
+
+/* One layer's page pool on the device. Row (page, head, slot) of head_dim
+ * values starts at element page * page_stride + head * head_stride + slot *
+ * slot_stride of k and of v. Rows may lie in any order of the three but not
+ * over each other, and each starts on 16 bytes (E_INVALID otherwise).
+ * head_dim: a multiple of 8, at most 128. */
+typedef struct {
+    void* k;
+    void* v;
+    uint32_t kv_f16;            /* 0 = f32, 1 = binary16 */
+    uint32_t num_pages, page_size, num_kv_heads, head_dim;
+    uint64_t page_stride, head_stride, slot_stride;
+} qora_paged_kv;
+
+/* A batch: sequence s has the rows row_start[s] .. row_start[s + 1] - 1 of the
+ * calls' row arrays (none if the two are equal), the last of its kv_len[s]
+ * cached positions; position p is slot p % page_size of page
+ * pages[s * max_pages + p / page_size]. The three arrays are on the device.
+ * Rows from row_start[num_seqs] on belong to nobody and are left as they are.
+ * Row offsets ascend from 0 to at most `rows`; offsets that do not, page ids
+ * outside the pool and lengths past the table reach no memory outside the
+ * arrays: what they describe is skipped. */
+typedef struct {
+    const int32_t* row_start;   /* [num_seqs + 1] */
+    const int32_t* kv_len;      /* [num_seqs], the new rows included */
+    const int32_t* pages;       /* [num_seqs][max_pages] */
+    uint32_t num_seqs, max_pages;
+    uint32_t rows;              /* rows of the calls' row arrays */
+    uint32_t max_new;           /* the most rows of one sequence (0: rows); qora_hip_paged_attn_run
+                                   computes no further row of a sequence */
+} qora_paged_batch;
+
+/* apply_rope_raw (gemv.rs:757-778) and the cache append (gemv.rs:1062-1083)
+ * of every row of the batch at its own position. q [rows][num_heads][head_dim],
+ * k and v [rows][num_kv_heads][head_dim], rows q_stride, k_stride, v_stride
+ * floats apart (the three may be parts of one q|k|v row). q and k are rotated
+ * with row `position` of cos_t, sin_t [rope_positions][half_dim] (half_dim 0:
+ * not rotated); q goes to q_out, rows q_out_stride floats apart, which may be
+ * q itself with the same stride; q and q_out both NULL: keys and values only.
+ * A row whose position has no page or no row of the tables is skipped: q_out
+ * and the cache stay as they were. Row pointers and strides are multiples of
+ * 16 bytes. Two rows of one position and sequence page race. */
+int qora_hip_paged_append(qora_hip_ctx* ctx, const qora_paged_kv* kv, const qora_paged_batch* batch,
+                          uint32_t num_heads, const float* q, uint64_t q_stride, const float* k, uint64_t k_stride,
+                          const float* v, uint64_t v_stride, float* q_out, uint64_t q_out_stride, const float* cos_t,
+                          const float* sin_t, uint32_t half_dim, uint64_t rope_positions, void* stream);
+
+/* Causal attention of the batch's rows over the paged cache (raw_prefill's and
+ * forward_decode_raw's, gemv.rs:914-989, 1088-1130): the row at position p
+ * attends to positions 0 .. p of its sequence, with scores q.k / sqrt(head_dim);
+ * a position on a page id outside the pool is not there, and a row that sees
+ * no position gets zeros. What positions a row does not see hold, NaN included,
+ * does not reach it. q and out: [rows][num_heads][head_dim], rows q_stride and
+ * out_stride floats apart; out may be q with the same stride, and may not
+ * overlap it otherwise.
+ * prepare allocates the workspace of calls of up to max_rows rows and max_seqs
+ * sequences; release frees it (both refused during capture). Calls with one id,
+ * graph replays included, use its workspace and must run one behind the
+ * other; work on several streams takes an id for each. */
+int qora_hip_paged_attn_prepare(qora_hip_ctx* ctx, uint32_t max_rows, uint32_t max_seqs, uint32_t num_heads,
+                                uint32_t num_kv_heads, uint32_t head_dim, uint32_t* attn_id);
+int qora_hip_paged_attn_run(qora_hip_ctx* ctx, uint32_t attn_id, const qora_paged_kv* kv,
+                            const qora_paged_batch* batch, const float* q, uint64_t q_stride, float* out,
+                            uint64_t out_stride, void* stream);
+int qora_hip_paged_attn_release(qora_hip_ctx* ctx, uint32_t attn_id);
+
+/* A low-rank adapter of a [k][n] projection: a [k][rank] and b [rank][n] in
+ * binary16, on the host (copied by the upload). */
+typedef struct {
+    const uint16_t* a;
+    const uint16_t* b;
+    uint32_t rank;              /* 1 .. 256 */
+    float scale;
+} qora_lora_adapter;
+
+/* qora_hip_gemm with an adapter of each row's own beside it:
+ * y[t] = x[t] . W + scale_e (x[t] . A_e) . B_e, e = row_adapter[t] (a device
+ * array of `rows` ids); an id outside 0 .. count - 1 means no adapter.
+ * lora_upload packs `count` adapters (1 .. 65536) of [k][n] projections once
+ * and allocates the workspace of calls of up to max_rows rows; lora_release
+ * frees both (refused during capture). The weight's k and n must be the
+ * adapters', n a multiple of 32 as in every upload. Calls with one lora id, and qora_hip_gemm's
+ * scratch in the context, as there: one behind the other. y may be x. */
+int qora_hip_lora_upload(qora_hip_ctx* ctx, const qora_lora_adapter* adapters, uint32_t count, uint64_t k, uint64_t n,
+                         uint32_t max_rows, uint32_t* lora_id);
+int qora_hip_lora_release(qora_hip_ctx* ctx, uint32_t lora_id);
+int qora_hip_gemm_lora(qora_hip_ctx* ctx, uint32_t wid, uint32_t lora_id, const float* x, float* y, uint64_t rows,
+                       const int32_t* row_adapter, void* stream);
+
 /* ---- synthetic inputs (host only; no device needed) ----------------------
  * Seeded, counter-based generator (splitmix64 streams keyed by seed and
  * tensor id) for the benchmark configurations. The reference has no

@@ -67,6 +67,27 @@ class HostModel(ctypes.Structure):
     ]
 
 
+class PagedKV(ctypes.Structure):
+    """qora_paged_kv: one layer's page pool (device addresses, strides in elements)."""
+
+    _fields_ = [("k", _P), ("v", _P), ("kv_f16", _U32), ("num_pages", _U32), ("page_size", _U32),
+                ("num_kv_heads", _U32), ("head_dim", _U32), ("page_stride", _U64), ("head_stride", _U64),
+                ("slot_stride", _U64)]
+
+
+class PagedBatch(ctypes.Structure):
+    """qora_paged_batch: the rows, lengths and page tables of a batch (device addresses)."""
+
+    _fields_ = [("row_start", _P), ("kv_len", _P), ("pages", _P), ("num_seqs", _U32), ("max_pages", _U32),
+                ("rows", _U32), ("max_new", _U32)]
+
+
+class LoraAdapterDesc(ctypes.Structure):
+    """qora_lora_adapter (host pointers)."""
+
+    _fields_ = [("a", _P), ("b", _P), ("rank", _U32), ("scale", _F)]
+
+
 SIGNATURES = {
     "qora_hip_create": (_I, [_I, ctypes.POINTER(_P)]),
     "qora_hip_destroy": (_I, [_P]),
@@ -118,6 +139,13 @@ SIGNATURES = {
     "qora_hip_attn_decode": (_I, [_P, _P, _P, _P, _I, _U32, _U32, _U32, _U32, _P, _P]),
     "qora_hip_gemm": (_I, [_P, _U32, _P, _P, _U64, _P]),
     "qora_hip_attn_prefill": (_I, [_P, _P, _P, _P, _I, _U32, _U32, _U32, _U32, _U32, _P, _P]),
+    "qora_hip_paged_append": (_I, [_P, _P, _P, _U32, _P, _U64, _P, _U64, _P, _U64, _P, _U64, _P, _P, _U32, _U64, _P]),
+    "qora_hip_paged_attn_prepare": (_I, [_P, _U32, _U32, _U32, _U32, _U32, _P]),
+    "qora_hip_paged_attn_run": (_I, [_P, _U32, _P, _P, _P, _U64, _P, _U64, _P]),
+    "qora_hip_paged_attn_release": (_I, [_P, _U32]),
+    "qora_hip_lora_upload": (_I, [_P, _P, _U32, _U64, _U64, _U32, _P]),
+    "qora_hip_lora_release": (_I, [_P, _U32]),
+    "qora_hip_gemm_lora": (_I, [_P, _U32, _U32, _P, _P, _U64, _P, _P]),
     "qora_hip_sample": (_I, [_P, _P, _U64, _P, _U64, _P, _P, _P, _P]),
     "qora_hip_decode_sample": (_I, [_P, _U32, _P, _U64, _P, _P, _P, _P]),
     "qora_hip_argmax": (_I, [_P, _P, _U64, _P, _P]),
@@ -250,6 +278,15 @@ class Weight:
 
 
 @dataclass
+class LoraAdapter:
+    """A low-rank adapter of a [k][n] projection: a [k][rank], b [rank][n]."""
+
+    a: np.ndarray
+    b: np.ndarray
+    scale: float = 1.0
+
+
+@dataclass
 class DecodeWeights:
     """Host-side mirror of DecodeWeights (gemv.rs:195-206)."""
 
@@ -360,6 +397,7 @@ class HipContext:
         if rc != QORA_HIP_OK:
             raise QoraHipError(rc, f"qora_hip_create(device={device}) failed (no usable HIP device?)")
         self.h = h.value
+        self._paged_heads = {}     # paged attention id -> query heads (its default row stride)
 
     def check(self, rc: int, what: str = "") -> None:
         if rc != QORA_HIP_OK:
@@ -465,6 +503,64 @@ class HipContext:
                                             ctypes.byref(params), ctypes.byref(st), ctypes.byref(tok), None),
                    "sample")
         return tok.value, st.value
+
+    # -- many requests -------------------------------------------------------
+    def paged_append(self, kv: "PagedKV", batch: "PagedBatch", num_heads: int, q: int, k: int, v: int, stride: int,
+                     q_out: int, cos: int = 0, sin: int = 0, half_dim: int = 0, rope_positions: int = 0,
+                     q_out_stride: int = 0, k_stride: int = 0, v_stride: int = 0, stream: int = 0) -> None:
+        """Rotates the batch's q and k rows and stores k and v in the paged cache
+        (device addresses; `stride` floats between rows of q, and of k and v unless
+        given; q_out's rows are num_heads * head_dim apart unless given)."""
+        self.check(self.lib.qora_hip_paged_append(
+            self.h, ctypes.byref(kv), ctypes.byref(batch), num_heads, q or None, stride, k, k_stride or stride, v,
+            v_stride or stride, q_out or None, q_out_stride or num_heads * kv.head_dim, cos or None, sin or None,
+            half_dim, rope_positions, stream or None), "paged_append")
+
+    def paged_attn_prepare(self, max_rows: int, max_seqs: int, num_heads: int, num_kv_heads: int,
+                           head_dim: int) -> int:
+        """Workspace of paged attention calls of up to that size; returns its id."""
+        aid = ctypes.c_uint32()
+        self.check(self.lib.qora_hip_paged_attn_prepare(self.h, max_rows, max_seqs, num_heads, num_kv_heads, head_dim,
+                                                        ctypes.byref(aid)), "paged_attn_prepare")
+        self._paged_heads[aid.value] = num_heads
+        return aid.value
+
+    def paged_attn_run(self, attn_id: int, kv: "PagedKV", batch: "PagedBatch", q: int, out: int, q_stride: int = 0,
+                       out_stride: int = 0, stream: int = 0) -> None:
+        """Causal attention of the batch's rows over the paged cache (device
+        addresses; rows num_heads * head_dim floats apart unless given)."""
+        row = self._paged_heads.get(attn_id, 0) * kv.head_dim
+        self.check(self.lib.qora_hip_paged_attn_run(self.h, attn_id, ctypes.byref(kv), ctypes.byref(batch), q,
+                                                    q_stride or row, out, out_stride or row, stream or None),
+                   "paged_attn_run")
+
+    def paged_attn_release(self, attn_id: int) -> None:
+        self.check(self.lib.qora_hip_paged_attn_release(self.h, attn_id), "paged_attn_release")
+
+    def lora_upload(self, adapters: Sequence["LoraAdapter"], max_rows: int) -> int:
+        """Packs the adapters of one projection; returns the id gemm_lora takes."""
+        keep, k, n = [], None, None
+        descs = (LoraAdapterDesc * len(adapters))()
+        for i, ad in enumerate(adapters):
+            a, b = (np.ascontiguousarray(m, dtype=np.float16) for m in (ad.a, ad.b))
+            if a.ndim != 2 or b.ndim != 2 or a.shape[1] != b.shape[0] or (k, n) not in ((None, None),
+                                                                                         (a.shape[0], b.shape[1])):
+                raise ValueError("adapters need a [k][rank] and b [rank][n] of the same k and n")
+            k, n = a.shape[0], b.shape[1]
+            keep += [a, b]
+            descs[i] = LoraAdapterDesc(_ptr(a), _ptr(b), a.shape[1], ad.scale)
+        lid = ctypes.c_uint32()
+        self.check(self.lib.qora_hip_lora_upload(self.h, descs, len(adapters), k or 0, n or 0, max_rows,
+                                                 ctypes.byref(lid)), "lora_upload")
+        return lid.value
+
+    def lora_release(self, lora_id: int) -> None:
+        self.check(self.lib.qora_hip_lora_release(self.h, lora_id), "lora_release")
+
+    def gemm_lora(self, wid: int, lora_id: int, x: int, y: int, rows: int, row_adapter: int, stream: int = 0) -> None:
+        """y = x . W plus each row's own adapter (device addresses)."""
+        self.check(self.lib.qora_hip_gemm_lora(self.h, wid, lora_id, x, y, rows, row_adapter, stream or None),
+                   "gemm_lora")
 
     def weight_ptrs(self, wid: int):
         a, b = ctypes.c_void_p(), ctypes.c_void_p()

@@ -2,6 +2,7 @@
 // KV cache, captured decode step, and kernel-level entry points.
 #include "../../include/qora_hip.h"
 #include "launch.hpp"
+#include "paged_args.hpp"
 
 #include <algorithm>
 #include <atomic>
@@ -190,6 +191,20 @@ struct PreparedGemv {
 constexpr size_t kPfAttnOneCounts = kPfAttnOneRows / 64 / 2;
 constexpr size_t kPfAttnOneBytes = (size_t)kPfAttnOneRows * (128 + 2) * sizeof(float);
 
+// Workspace of paged attention calls (qora_hip_paged_attn_prepare).
+struct PagedAttnWs {
+    bool alive = false;
+    uint32_t max_rows = 0, max_seqs = 0, H = 0, KVH = 0, hd = 0;
+};
+
+// Packed adapters and their workspace (qora_hip_lora_upload).
+struct LoraSet {
+    bool alive = false;
+    uint32_t count = 0, k = 0, n = 0, rp = 0, max_rows = 0;
+    void* mem = nullptr;       // entries, then every adapter's at and bt
+    float* u = nullptr;        // x . A
+};
+
 struct qora_hip_ctx {
     int device = 0;
     hipStream_t stream = nullptr;
@@ -243,6 +258,8 @@ struct qora_hip_ctx {
     bool capturing = false;
     bool tok_armed = false;              // h_tok[0] set to kTokPending for the step in flight
     std::vector<PreparedGemv> gemvs;
+    std::vector<PagedAttnWs> pattns;
+    std::vector<LoraSet> loras;
     ModelState m;
 };
 
@@ -625,6 +642,9 @@ extern "C" int qora_hip_destroy(qora_hip_ctx* c) {
     free_model(c);
     for (PreparedGemv& g : c->gemvs)
         for (void* q : {g.tw, g.ts, g.te, g.part_val, g.part_idx})
+            if (q) (void)hipFree(q);
+    for (LoraSet& a : c->loras)
+        for (void* q : {a.mem, (void*)a.u})
             if (q) (void)hipFree(q);
     for (DevWeight& w : c->weights) {
         if (w.w) (void)hipFree(w.w);
@@ -2622,4 +2642,315 @@ extern "C" int qora_hip_argmax(qora_hip_ctx* c, const float* logits, uint64_t n,
     if (n == 0 || n > 0x7FFFFFFFull) return fail(c, QORA_HIP_E_INVALID, "bad length");
     HIP_TRY(c, launch_argmax(logits, (uint32_t)n, out, pick_stream(c, stream)));
     return QORA_HIP_OK;
+}
+
+// ===========================================================================
+// many requests at once: paged KV cache, low-rank adapters
+// ===========================================================================
+
+namespace {
+
+// The context's device for the duration of a call, whichever one the caller's
+// thread has current.
+struct DeviceGuard {
+    int old = -1;
+    hipError_t err;
+    explicit DeviceGuard(int device) {
+        err = hipGetDevice(&old);
+        if (err == hipSuccess && old != device) err = hipSetDevice(device);
+        else old = -1;
+    }
+    ~DeviceGuard() {
+        if (old >= 0) (void)hipSetDevice(old);
+    }
+};
+
+// Whether a call that allocates or frees would touch a recording: the context's own
+// capture, or the caller's on the context's stream.
+int not_captured(qora_hip_ctx* c, const char* what) {
+    if (!captured(c, c->stream)) return QORA_HIP_OK;
+    return fail(c, QORA_HIP_E_STATE, std::string(what) + ": not allowed during capture");
+}
+
+PagedParams paged_params(const qora_paged_kv* kv, const qora_paged_batch* b) {
+    PagedParams g{};
+    g.k = kv->k;
+    g.v = kv->v;
+    g.page_stride = kv->page_stride;
+    g.head_stride = kv->head_stride;
+    g.slot_stride = kv->slot_stride;
+    g.num_pages = kv->num_pages;
+    g.page_size = kv->page_size;
+    g.KVH = kv->num_kv_heads;
+    g.hd = kv->head_dim;
+    g.row_start = b->row_start;
+    g.kv_len = b->kv_len;
+    g.pages = b->pages;
+    g.seqs = b->num_seqs;
+    g.max_pages = b->max_pages;
+    g.rows = b->rows;
+    g.max_new = b->max_new ? std::min(b->max_new, b->rows) : b->rows;
+    return g;
+}
+
+// Bytes from the first to the last element of `rows` rows.
+uint64_t rows_bytes(uint64_t rows, uint64_t ld, uint64_t width) { return rows ? ((rows - 1) * ld + width) * 4 : 0; }
+
+// No exception leaves a C entry: what the host's own containers throw (no
+// memory) is reported as such.
+template <typename F>
+int no_throw(F body) {
+    try {
+        return body();
+    } catch (...) {
+        return QORA_HIP_E_NOMEM;
+    }
+}
+
+}  // namespace
+
+extern "C" int qora_hip_paged_append(qora_hip_ctx* c, const qora_paged_kv* kv, const qora_paged_batch* batch,
+                                     uint32_t num_heads, const float* q, uint64_t q_stride, const float* k,
+                                     uint64_t k_stride, const float* v, uint64_t v_stride, float* q_out,
+                                     uint64_t q_out_stride, const float* cos_t, const float* sin_t, uint32_t half_dim,
+                                     uint64_t rope_positions, void* stream) {
+    if (!c) return QORA_HIP_E_INVALID;
+    return no_throw([&]() -> int {
+        const char* e = paged_kv_error(kv);
+        if (!e) e = paged_batch_error(kv, batch);
+        if (e) return fail(c, QORA_HIP_E_INVALID, e);
+        const uint32_t hd = kv->head_dim;
+        if (half_dim > hd / 2) return fail(c, QORA_HIP_E_INVALID, "half_dim exceeds head_dim / 2");
+        if (half_dim && (!cos_t || !sin_t || rope_positions == 0)) return fail(c, QORA_HIP_E_INVALID, "null rotation table");
+        if ((q != nullptr) != (q_out != nullptr)) return fail(c, QORA_HIP_E_INVALID, "q and q_out come together");
+        if (batch->rows == 0 || batch->num_seqs == 0) return QORA_HIP_OK;
+        if (q && (num_heads == 0 || num_heads > 65535u)) return fail(c, QORA_HIP_E_INVALID, "bad head count");
+        if (q) {
+            e = paged_rows_error(q, q_stride, num_heads, hd);
+            if (!e) e = paged_rows_error(q_out, q_out_stride, num_heads, hd);
+        }
+        if (!e) e = paged_rows_error(k, k_stride, kv->num_kv_heads, hd);
+        if (!e) e = paged_rows_error(v, v_stride, kv->num_kv_heads, hd);
+        if (e) return fail(c, QORA_HIP_E_INVALID, e);
+        if (q && !(q == q_out && q_stride == q_out_stride) &&
+            overlap(q, rows_bytes(batch->rows, q_stride, (uint64_t)num_heads * hd), q_out,
+                    rows_bytes(batch->rows, q_out_stride, (uint64_t)num_heads * hd)))
+            return fail(c, QORA_HIP_E_INVALID, "q_out overlaps q");
+        PagedAppendParams p{};
+        p.g = paged_params(kv, batch);
+        p.q = q;
+        p.kin = k;
+        p.vin = v;
+        p.q_out = q_out;
+        p.ldq = q_stride;
+        p.ldk = k_stride;
+        p.ldv = v_stride;
+        p.ldqo = q_out_stride;
+        p.cos_t = cos_t;
+        p.sin_t = sin_t;
+        p.H = num_heads;
+        p.half = half_dim;
+        p.rope_positions = rope_positions;
+        DeviceGuard dev(c->device);
+        HIP_TRY(c, dev.err);
+        HIP_TRY(c, launch_paged_append(p, kv->kv_f16 != 0, pick_stream(c, stream)));
+        return QORA_HIP_OK;
+    });
+}
+
+extern "C" int qora_hip_paged_attn_prepare(qora_hip_ctx* c, uint32_t max_rows, uint32_t max_seqs, uint32_t num_heads,
+                                           uint32_t num_kv_heads, uint32_t head_dim, uint32_t* attn_id) {
+    if (!c) return QORA_HIP_E_INVALID;
+    return no_throw([&]() -> int {
+        if (!attn_id) return fail(c, QORA_HIP_E_INVALID, "null argument");
+        if (max_rows == 0 || max_rows > 0x7FFFFFFFu || max_seqs == 0 || max_seqs > kPagedMaxSeqs)
+            return fail(c, QORA_HIP_E_INVALID, "bad row or sequence count");
+        if (num_heads == 0 || num_kv_heads == 0 || num_heads % num_kv_heads != 0 || num_heads > 65535u || head_dim == 0 ||
+            head_dim > 128 || head_dim % 8 != 0)
+            return fail(c, QORA_HIP_E_INVALID, "attention needs H % KVH == 0, head_dim <= 128 and a multiple of 8");
+        if (int rc = not_captured(c, "paged_attn_prepare allocates")) return rc;
+        PagedAttnWs w;
+        w.max_rows = max_rows;
+        w.max_seqs = max_seqs;
+        w.H = num_heads;
+        w.KVH = num_kv_heads;
+        w.hd = head_dim;
+        w.alive = true;
+        c->pattns.push_back(w);
+        *attn_id = (uint32_t)(c->pattns.size() - 1);
+        return QORA_HIP_OK;
+    });
+}
+
+extern "C" int qora_hip_paged_attn_run(qora_hip_ctx* c, uint32_t attn_id, const qora_paged_kv* kv,
+                                       const qora_paged_batch* batch, const float* q, uint64_t q_stride, float* out,
+                                       uint64_t out_stride, void* stream) {
+    if (!c) return QORA_HIP_E_INVALID;
+    return no_throw([&]() -> int {
+        if (attn_id >= c->pattns.size() || !c->pattns[attn_id].alive)
+            return fail(c, QORA_HIP_E_INVALID, "unknown paged attention id");
+        const PagedAttnWs& w = c->pattns[attn_id];
+        const char* e = paged_kv_error(kv);
+        if (!e) e = paged_batch_error(kv, batch);
+        if (e) return fail(c, QORA_HIP_E_INVALID, e);
+        if (kv->num_kv_heads != w.KVH || kv->head_dim != w.hd)
+            return fail(c, QORA_HIP_E_INVALID, "cache heads differ from the prepared ones");
+        if (batch->rows > w.max_rows || batch->num_seqs > w.max_seqs)
+            return fail(c, QORA_HIP_E_INVALID, "batch is larger than the prepared workspace");
+        if (batch->rows == 0 || batch->num_seqs == 0) return QORA_HIP_OK;
+        e = paged_rows_error(q, q_stride, w.H, w.hd);
+        if (!e) e = paged_rows_error(out, out_stride, w.H, w.hd);
+        if (e) return fail(c, QORA_HIP_E_INVALID, e);
+        const uint64_t width = (uint64_t)w.H * w.hd;
+        if (!(q == out && q_stride == out_stride) &&
+            overlap(q, rows_bytes(batch->rows, q_stride, width), out, rows_bytes(batch->rows, out_stride, width)))
+            return fail(c, QORA_HIP_E_INVALID, "out overlaps q");
+        PagedAttnParams p{};
+        p.g = paged_params(kv, batch);
+        p.q = q;
+        p.out = out;
+        p.ldq = q_stride;
+        p.ldo = out_stride;
+        p.H = w.H;
+        p.G = w.H / w.KVH;
+        p.scale = 1.0f / sqrtf((float)w.hd);
+        DeviceGuard dev(c->device);
+        HIP_TRY(c, dev.err);
+        HIP_TRY(c, launch_paged_attn(p, kv->kv_f16 != 0, pick_stream(c, stream)));
+        return QORA_HIP_OK;
+    });
+}
+
+extern "C" int qora_hip_paged_attn_release(qora_hip_ctx* c, uint32_t attn_id) {
+    if (!c) return QORA_HIP_E_INVALID;
+    return no_throw([&]() -> int {
+        if (attn_id >= c->pattns.size() || !c->pattns[attn_id].alive)
+            return fail(c, QORA_HIP_E_INVALID, "unknown paged attention id");
+        if (int rc = not_captured(c, "paged_attn_release frees")) return rc;
+        c->pattns[attn_id] = PagedAttnWs();
+        return QORA_HIP_OK;
+    });
+}
+
+extern "C" int qora_hip_lora_upload(qora_hip_ctx* c, const qora_lora_adapter* ad, uint32_t count, uint64_t k,
+                                    uint64_t n, uint32_t max_rows, uint32_t* lora_id) {
+    if (!c) return QORA_HIP_E_INVALID;
+    return no_throw([&]() -> int {
+        if (!ad || !lora_id) return fail(c, QORA_HIP_E_INVALID, "null argument");
+        if (count == 0 || count > 65536u || max_rows == 0 || max_rows > 0x7FFFFFFFu)
+            return fail(c, QORA_HIP_E_INVALID, "bad adapter or row count");
+        if (k == 0 || n == 0 || k % 32 != 0 || n % 32 != 0 || k > 0x7FFFFFFFull || n > 0x7FFFFFFFull)
+            return fail(c, QORA_HIP_E_INVALID, "adapters need k and n multiples of 32");
+        for (uint32_t i = 0; i < count; ++i) {
+            if (!ad[i].a || !ad[i].b) return fail(c, QORA_HIP_E_INVALID, "null adapter matrix");
+            if (ad[i].rank == 0 || ad[i].rank > 256u) return fail(c, QORA_HIP_E_INVALID, "adapter rank must be 1 .. 256");
+        }
+        if (int rc = not_captured(c, "lora_upload allocates")) return rc;
+        LoraSet s;
+        s.count = count;
+        s.k = (uint32_t)k;
+        s.n = (uint32_t)n;
+        s.max_rows = max_rows;
+        const uint64_t head = al256((uint64_t)count * sizeof(LoraEntry));
+        uint64_t bytes = head;
+        for (uint32_t i = 0; i < count; ++i) {
+            const uint32_t rp = (ad[i].rank + 15u) & ~15u;
+            s.rp = std::max(s.rp, rp);
+            bytes += 2u * rp * (k + n);
+        }
+        c->loras.reserve(c->loras.size() + 1);
+        std::vector<LoraEntry> entries(count);
+        std::vector<uint16_t> host;
+        DeviceGuard dev(c->device);
+        HIP_TRY(c, dev.err);
+        if (int rc = dalloc(c, bytes, &s.mem)) return rc;
+        auto drop = [&]() {
+            for (void* p : {s.mem, (void*)s.u})
+                if (p) (void)hipFree(p);
+        };
+        hipError_t e = hipSuccess;
+        try {
+            if (int rc = dalloc(c, (uint64_t)max_rows * s.rp * sizeof(float), (void**)&s.u)) {
+                drop();
+                return rc;
+            }
+            uint64_t at = head;
+            for (uint32_t i = 0; i < count && e == hipSuccess; ++i) {
+                // at[r][k] and bt[n][r], ranks past the adapter's own zero
+                const uint32_t r = ad[i].rank;
+                const uint32_t rp = (r + 15u) & ~15u;
+                host.assign((size_t)rp * (k + n), 0);
+                for (uint64_t j = 0; j < k; ++j)
+                    for (uint32_t x = 0; x < r; ++x) host[x * k + j] = ad[i].a[j * r + x];
+                uint16_t* bt = host.data() + (size_t)rp * k;
+                for (uint32_t x = 0; x < r; ++x)
+                    for (uint64_t j = 0; j < n; ++j) bt[j * rp + x] = ad[i].b[x * n + j];
+                uint8_t* d = (uint8_t*)s.mem + at;
+                entries[i] = LoraEntry{(const uint16_t*)d, (const uint16_t*)(d + 2u * rp * k), rp, ad[i].scale};
+                e = hipMemcpy(d, host.data(), host.size() * 2, hipMemcpyHostToDevice);
+                at += host.size() * 2;
+            }
+            if (e == hipSuccess) e = hipMemcpy(s.mem, entries.data(), count * sizeof(LoraEntry), hipMemcpyHostToDevice);
+        } catch (...) {
+            drop();
+            return QORA_HIP_E_NOMEM;
+        }
+        if (e != hipSuccess) {
+            drop();
+            return fail(c, QORA_HIP_E_DEVICE, std::string("adapter upload: ") + hipGetErrorString(e));
+        }
+        s.alive = true;
+        c->loras.push_back(s);
+        *lora_id = (uint32_t)(c->loras.size() - 1);
+        return QORA_HIP_OK;
+    });
+}
+
+extern "C" int qora_hip_lora_release(qora_hip_ctx* c, uint32_t lora_id) {
+    if (!c) return QORA_HIP_E_INVALID;
+    return no_throw([&]() -> int {
+        if (lora_id >= c->loras.size() || !c->loras[lora_id].alive) return fail(c, QORA_HIP_E_INVALID, "unknown lora id");
+        if (int rc = not_captured(c, "lora_release frees")) return rc;
+        DeviceGuard dev(c->device);
+        HIP_TRY(c, dev.err);
+        HIP_TRY(c, hipStreamSynchronize(c->stream));
+        LoraSet& s = c->loras[lora_id];
+        for (void* p : {s.mem, (void*)s.u})
+            if (p) (void)hipFree(p);
+        s = LoraSet();
+        return QORA_HIP_OK;
+    });
+}
+
+extern "C" int qora_hip_gemm_lora(qora_hip_ctx* c, uint32_t wid, uint32_t lora_id, const float* x, float* y,
+                                  uint64_t rows, const int32_t* row_adapter, void* stream) {
+    if (!c) return QORA_HIP_E_INVALID;
+    return no_throw([&]() -> int {
+        if (!x || !y || !row_adapter) return fail(c, QORA_HIP_E_INVALID, "null argument");
+        if (lora_id >= c->loras.size() || !c->loras[lora_id].alive) return fail(c, QORA_HIP_E_INVALID, "unknown lora id");
+        const LoraSet& s = c->loras[lora_id];
+        const DevWeight* w = get_weight(c, wid);
+        if (!w) return fail(c, QORA_HIP_E_INVALID, "unknown weight id");
+        if (w->k != s.k || w->n != s.n) return fail(c, QORA_HIP_E_INVALID, "weight and adapters differ in shape");
+        if (rows == 0 || rows > s.max_rows) return fail(c, QORA_HIP_E_INVALID, "more rows than the adapters' workspace holds");
+        DeviceGuard dev(c->device);
+        HIP_TRY(c, dev.err);
+        const hipStream_t st = pick_stream(c, stream);
+        LoraParams p{};
+        p.entries = (const LoraEntry*)s.mem;
+        p.count = s.count;
+        p.k = s.k;
+        p.n = s.n;
+        p.rows = (uint32_t)rows;
+        p.rp = s.rp;
+        p.row_adapter = row_adapter;
+        p.x = x;
+        p.y = y;
+        p.u = s.u;
+        // x . A before the product, which may write y over x
+        HIP_TRY(c, launch_lora_shrink(p, st));
+        if (int rc = qora_hip_gemm(c, wid, x, y, rows, stream)) return rc;
+        HIP_TRY(c, launch_lora_expand(p, st));
+        return QORA_HIP_OK;
+    });
 }

@@ -173,4 +173,10 @@ uint32_t smp_sort_keys(uint32_t vocab);
 bool smp_sort_supported(uint32_t vocab);
 hipError_t launch_sample_sorted(const float* logits, const SampleParams& p, uint32_t k, hipStream_t stream);
 
+// many requests (paged.hpp, lora.hpp)
+hipError_t launch_paged_append(const PagedAppendParams& p, bool f16, hipStream_t stream);
+hipError_t launch_paged_attn(const PagedAttnParams& p, bool f16, hipStream_t stream);
+hipError_t launch_lora_shrink(const LoraParams& p, hipStream_t stream);
+hipError_t launch_lora_expand(const LoraParams& p, hipStream_t stream);
+
 }  // namespace qora

@@ -405,4 +405,59 @@ struct EmbedParams {
     long long* xacc;         // fixed-point residual stream, set (not added)
 };
 
+// Paged cache and batch of the many-request calls (qora_paged_kv, qora_paged_batch).
+struct PagedParams {
+    void* k;
+    void* v;
+    uint64_t page_stride, head_stride, slot_stride;   // elements
+    uint32_t num_pages, page_size, KVH, hd;
+    const int32_t* row_start;
+    const int32_t* kv_len;
+    const int32_t* pages;
+    uint32_t seqs, max_pages, rows, max_new;
+};
+
+struct PagedAppendParams {
+    PagedParams g;
+    const float* q;            // nullptr: keys and values only
+    const float* kin;
+    const float* vin;
+    float* q_out;
+    uint64_t ldq, ldk, ldv, ldqo;
+    const float* cos_t;
+    const float* sin_t;
+    uint32_t H, half;
+    uint64_t rope_positions;
+    uint32_t units;            // 4-dim units of a row
+};
+
+struct PagedAttnParams {
+    PagedParams g;
+    const float* q;
+    float* out;
+    uint64_t ldq, ldo;
+    uint32_t H, G;             // query heads, of one KV head
+    float scale;               // 1 / sqrt(hd)
+};
+
+// Low-rank adapters of a [k][n] projection, packed by the upload: at[e] is A
+// transposed [rp][k], bt[e] is B transposed [n][rp], rp = rank rounded up to 16
+// with zeros.
+struct LoraEntry {
+    const uint16_t* at;
+    const uint16_t* bt;
+    uint32_t rp;
+    float scale;
+};
+
+struct LoraParams {
+    const LoraEntry* entries;
+    uint32_t count, k, n, rows;
+    uint32_t rp;               // the largest rp
+    const int32_t* row_adapter;
+    const float* x;
+    float* y;
+    float* u;                  // [rows][rp]: x . A
+};
+
 }  // namespace qora

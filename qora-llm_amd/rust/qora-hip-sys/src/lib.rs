@@ -78,6 +78,47 @@ pub struct qora_sample_params {
     pub presence_penalty: f32,
 }
 
+/// One layer's page pool of many requests' keys and values (device pointers, strides in elements).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct qora_paged_kv {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    /// 0 = f32, 1 = binary16
+    pub kv_f16: u32,
+    pub num_pages: u32,
+    pub page_size: u32,
+    pub num_kv_heads: u32,
+    pub head_dim: u32,
+    pub page_stride: u64,
+    pub head_stride: u64,
+    pub slot_stride: u64,
+}
+
+/// Rows, lengths and page tables of a batch (device pointers).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct qora_paged_batch {
+    pub row_start: *const i32,
+    pub kv_len: *const i32,
+    pub pages: *const i32,
+    pub num_seqs: u32,
+    pub max_pages: u32,
+    pub rows: u32,
+    /// the most rows of one sequence, 0: rows
+    pub max_new: u32,
+}
+
+/// A low-rank adapter: a [k][rank], b [rank][n] in binary16 (host pointers).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct qora_lora_adapter {
+    pub a: *const u16,
+    pub b: *const u16,
+    pub rank: u32,
+    pub scale: f32,
+}
+
 /// Host-side model for qora_file_write (the .qora v1 writer, save.rs:119-152).
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
@@ -211,6 +252,23 @@ extern "C" {
                                  out: *mut f32, stream: *mut c_void) -> c_int;
     pub fn qora_hip_argmax(ctx: *mut qora_hip_ctx, logits: *const f32, n: u64, out_device: *mut i32,
                            stream: *mut c_void) -> c_int;
+
+    // ---- many requests at once ----
+    pub fn qora_hip_paged_append(ctx: *mut qora_hip_ctx, kv: *const qora_paged_kv, batch: *const qora_paged_batch,
+                                 num_heads: u32, q: *const f32, q_stride: u64, k: *const f32, k_stride: u64,
+                                 v: *const f32, v_stride: u64, q_out: *mut f32, q_out_stride: u64, cos_t: *const f32,
+                                 sin_t: *const f32, half_dim: u32, rope_positions: u64, stream: *mut c_void) -> c_int;
+    pub fn qora_hip_paged_attn_prepare(ctx: *mut qora_hip_ctx, max_rows: u32, max_seqs: u32, num_heads: u32,
+                                       num_kv_heads: u32, head_dim: u32, attn_id: *mut u32) -> c_int;
+    pub fn qora_hip_paged_attn_run(ctx: *mut qora_hip_ctx, attn_id: u32, kv: *const qora_paged_kv,
+                                   batch: *const qora_paged_batch, q: *const f32, q_stride: u64, out: *mut f32,
+                                   out_stride: u64, stream: *mut c_void) -> c_int;
+    pub fn qora_hip_paged_attn_release(ctx: *mut qora_hip_ctx, attn_id: u32) -> c_int;
+    pub fn qora_hip_lora_upload(ctx: *mut qora_hip_ctx, adapters: *const qora_lora_adapter, count: u32, k: u64, n: u64,
+                                max_rows: u32, lora_id: *mut u32) -> c_int;
+    pub fn qora_hip_lora_release(ctx: *mut qora_hip_ctx, lora_id: u32) -> c_int;
+    pub fn qora_hip_gemm_lora(ctx: *mut qora_hip_ctx, wid: u32, lora_id: u32, x: *const f32, y: *mut f32, rows: u64,
+                              row_adapter: *const i32, stream: *mut c_void) -> c_int;
 
     // ---- host utilities (no device; no status) ----
     pub fn qora_synth_q4(seed: u64, tensor_id: u64, k: u64, n: u64, packed: *mut u8, scales: *mut u16);
