@@ -307,7 +307,8 @@ int qora_hip_argmax(qora_hip_ctx* ctx, const float* logits, uint64_t n, int32_t*
 /* One layer's page pool on the device. Row (page, head, slot) of head_dim
  * values starts at element page * page_stride + head * head_stride + slot *
  * slot_stride of k and of v. Rows may lie in any order of the three but not
- * over each other, and each starts on 16 bytes (E_INVALID otherwise).
+ * over each other, and each starts on 16 bytes (E_INVALID otherwise); k and v
+ * span at most 64 GiB each.
  * head_dim: a multiple of 8, at most 128. */
 typedef struct {
     void* k;

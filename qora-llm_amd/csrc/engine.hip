@@ -195,6 +195,8 @@ constexpr size_t kPfAttnOneBytes = (size_t)kPfAttnOneRows * (128 + 2) * sizeof(f
 struct PagedAttnWs {
     bool alive = false;
     uint32_t max_rows = 0, max_seqs = 0, H = 0, KVH = 0, hd = 0;
+    uint32_t* count = nullptr; // arrivals, zero between calls; the states behind them
+    float* part = nullptr;
 };
 
 // Packed adapters and their workspace (qora_hip_lora_upload).
@@ -643,6 +645,8 @@ extern "C" int qora_hip_destroy(qora_hip_ctx* c) {
     for (PreparedGemv& g : c->gemvs)
         for (void* q : {g.tw, g.ts, g.te, g.part_val, g.part_idx})
             if (q) (void)hipFree(q);
+    for (PagedAttnWs& a : c->pattns)
+        if (a.count) (void)hipFree(a.count);
     for (LoraSet& a : c->loras)
         for (void* q : {a.mem, (void*)a.u})
             if (q) (void)hipFree(q);
@@ -2775,6 +2779,25 @@ extern "C" int qora_hip_paged_attn_prepare(qora_hip_ctx* c, uint32_t max_rows, u
         w.H = num_heads;
         w.KVH = num_kv_heads;
         w.hd = head_dim;
+        const uint32_t G = num_heads / num_kv_heads;
+        const uint64_t items = paged_attn_items(max_rows, max_seqs, G, num_kv_heads, c->cus);
+        const uint64_t cb = al256(items * sizeof(uint32_t));
+        if (items > 0x7FFFFFFFull) return fail(c, QORA_HIP_E_INVALID, "bad row or sequence count");
+        c->pattns.reserve(c->pattns.size() + 1);
+        DeviceGuard dev(c->device);
+        HIP_TRY(c, dev.err);
+        void* mem;
+        if (int rc = dalloc(c, cb + paged_attn_part_bytes(max_rows, max_seqs, G, num_kv_heads, head_dim, c->cus), &mem))
+            return rc;
+        // (waited for: a call on another stream is not ordered behind the context's)
+        hipError_t e = hipMemsetAsync(mem, 0, cb, c->stream);
+        if (e == hipSuccess) e = hipStreamSynchronize(c->stream);
+        if (e != hipSuccess) {
+            (void)hipFree(mem);
+            return fail(c, QORA_HIP_E_DEVICE, std::string("paged attention workspace: ") + hipGetErrorString(e));
+        }
+        w.count = (uint32_t*)mem;
+        w.part = (float*)((uint8_t*)mem + cb);
         w.alive = true;
         c->pattns.push_back(w);
         *attn_id = (uint32_t)(c->pattns.size() - 1);
@@ -2814,9 +2837,11 @@ extern "C" int qora_hip_paged_attn_run(qora_hip_ctx* c, uint32_t attn_id, const 
         p.H = w.H;
         p.G = w.H / w.KVH;
         p.scale = 1.0f / sqrtf((float)w.hd);
+        p.part = w.part;
+        p.count = w.count;
         DeviceGuard dev(c->device);
         HIP_TRY(c, dev.err);
-        HIP_TRY(c, launch_paged_attn(p, kv->kv_f16 != 0, pick_stream(c, stream)));
+        HIP_TRY(c, launch_paged_attn(p, kv->kv_f16 != 0, c->cus, pick_stream(c, stream)));
         return QORA_HIP_OK;
     });
 }
@@ -2827,6 +2852,10 @@ extern "C" int qora_hip_paged_attn_release(qora_hip_ctx* c, uint32_t attn_id) {
         if (attn_id >= c->pattns.size() || !c->pattns[attn_id].alive)
             return fail(c, QORA_HIP_E_INVALID, "unknown paged attention id");
         if (int rc = not_captured(c, "paged_attn_release frees")) return rc;
+        DeviceGuard dev(c->device);
+        HIP_TRY(c, dev.err);
+        HIP_TRY(c, hipStreamSynchronize(c->stream));
+        if (c->pattns[attn_id].count) (void)hipFree(c->pattns[attn_id].count);
         c->pattns[attn_id] = PagedAttnWs();
         return QORA_HIP_OK;
     });

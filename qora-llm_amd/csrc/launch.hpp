@@ -175,7 +175,11 @@ hipError_t launch_sample_sorted(const float* logits, const SampleParams& p, uint
 
 // many requests (paged.hpp, lora.hpp)
 hipError_t launch_paged_append(const PagedAppendParams& p, bool f16, hipStream_t stream);
-hipError_t launch_paged_attn(const PagedAttnParams& p, bool f16, hipStream_t stream);
+// Items (workgroups, counters) and bytes of states of calls of up to that many rows and sequences.
+uint64_t paged_attn_items(uint64_t rows, uint64_t seqs, uint32_t G, uint32_t KVH, int cus);
+uint64_t paged_attn_part_bytes(uint64_t rows, uint64_t seqs, uint32_t G, uint32_t KVH, uint32_t hd, int cus);
+// p.part and p.count hold that; part_floats, the strides in units and the item costs are set here.
+hipError_t launch_paged_attn(const PagedAttnParams& p, bool f16, int cus, hipStream_t stream);
 hipError_t launch_lora_shrink(const LoraParams& p, hipStream_t stream);
 hipError_t launch_lora_expand(const LoraParams& p, hipStream_t stream);
 

@@ -124,75 +124,1040 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams p) 
 }
 
 // ---------------------------------------------------------------------------
-// Attention, one wave per (row, query head): 64 positions a step, a lane
-// scoring one of them, then the lanes over the dims.
+// Attention. The query rows of a sequence that share a KV head are flattened,
+// row i = token i / G of head i % G, so every group size fills the matrix
+// tiles alike, and are cut into tiles; a tile's keys are cut into chunks, and a
+// (sequence, chunk, tile, KV head) is one workgroup's item. What the item
+// numbers mean is worked out on the device from the batch's arrays by every
+// wave (two loads and a scan over the sequences, no second launch and no
+// host copy), with chunk lengths such that all items together are about
+// p.target of equal cost: a batch of one long request splits far, many
+// requests hardly, and a captured graph follows its arrays.
+//   Narrow items (at most 16 rows: single tokens): four waves walk the keys in
+//   turn, each with K and V of its own keys straight from the cache in
+//   registers, and join their states at the end.
+//   Wide items (128 rows): four waves of 32 rows share key tiles in LDS.
+// Both keep the running maximum and sum of each row's softmax in float32 and
+// hold the scores transposed (S^T = K Q^T, then O^T += V^T P^T), so that a row's
+// state lives in its own lanes and its weights never leave them.
+// Numerics: the matrix cores take two-byte operands. Over a binary16 cache K and V
+// are exact, q (on a power-of-two scale of its row) and the weights (times 2^15)
+// are split into two binary16 parts; over a float32 cache every operand is split
+// into three bfloat16 parts by cutting its bits (exact: 3 x 8 = 24), and the six
+// products above 2^-24 are kept. Sums are float32.
 // ---------------------------------------------------------------------------
-template <bool F16KV>
-__global__ __launch_bounds__(64) void paged_attn_row_kernel(PagedAttnParams p) {
-    __shared__ float qs[kAttnMaxHd];
-    __shared__ float es[kWave];
-    __shared__ uint64_t offs[kWave];
+typedef _Float16 pg_half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 pg_bf8 __attribute__((ext_vector_type(8)));
+typedef short pg_s4 __attribute__((ext_vector_type(4)));
+typedef float pg_f4 __attribute__((ext_vector_type(4)));
+typedef float pg_f16 __attribute__((ext_vector_type(16)));
+
+constexpr uint32_t kPgNarrowRows = 16, kPgWideRows = 128;
+// keys of a step: a narrow item's four waves, a wide item's tile
+__host__ __device__ constexpr uint32_t pg_narrow_keys(bool f16) { return f16 ? 128u : 64u; }
+__host__ __device__ constexpr uint32_t pg_wide_keys(bool f16) { return f16 ? 64u : 32u; }
+// floats of an item's state in the workspace
+__host__ __device__ constexpr uint32_t pg_part_floats(uint32_t HD, bool wide) {
+    return wide ? kPgWideRows * HD + 512u : kPgNarrowRows * HD + 32u;
+}
+
+struct PagedItem {
+    uint32_t s, kvh, tile, chunk;
+    uint32_t tiles, chunks;
+    uint32_t per;              // steps of a chunk
+    uint32_t first;            // item of the tile's chunk 0
+    uint32_t row0, n, len;     // the sequence's first row, its rows, keys any of them sees
+    int64_t pos0;              // position of its first row
+    bool narrow;
+};
+
+// A sequence's part of the plan.
+struct PagedSeqPlan {
+    uint32_t row0, n, len, tiles, steps;
+    int64_t pos0;
+    bool narrow;
+};
+
+__device__ __forceinline__ PagedSeqPlan paged_seq_plan(const PagedAttnParams& p, uint32_t s) {
     const PagedParams& g = p.g;
-    const uint32_t row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-    const uint32_t s = paged_seq_of(g, row);
-    const int32_t rb = g.row_start[s], re = g.row_start[s + 1u];
-    if (paged_rows_of(rb, re, g.rows) == 0 || (int32_t)row < rb || (int32_t)row >= re) return;
-    if (row - (uint32_t)rb >= g.max_new) return;
-    const int64_t pos = (int64_t)g.kv_len[s] - (re - (int32_t)row);
-    const uint32_t nk = (uint32_t)max((int64_t)0, min(pos + 1, (int64_t)g.page_size * g.max_pages));
-    const float* q = p.q + (uint64_t)row * p.ldq + (uint64_t)h * g.hd;
-    for (uint32_t d = lane; d < g.hd; d += kWave) qs[d] = q[d];
+    PagedSeqPlan q{};
+    const uint32_t c = min(s, g.seqs - 1u);
+    const int32_t a = g.row_start[c], b = g.row_start[c + 1u], L = g.kv_len[c];
+    const uint32_t all = s < g.seqs ? paged_rows_of(a, b, g.rows) : 0u;
+    q.n = min(all, g.max_new);
+    q.row0 = (uint32_t)a;
+    q.pos0 = (int64_t)L - (int64_t)all;
+    const int64_t cap = (int64_t)g.page_size * g.max_pages;
+    q.len = (uint32_t)max((int64_t)0, min(min((int64_t)L, cap), q.pos0 + (int64_t)q.n));
+    const uint64_t M = (uint64_t)q.n * p.G;
+    q.narrow = M <= kPgNarrowRows;
+    q.tiles = q.narrow ? (q.n ? 1u : 0u) : (uint32_t)((M + kPgWideRows - 1u) / kPgWideRows);
+    const uint32_t k = q.narrow ? p.narrow_keys : p.wide_keys;
+    q.steps = (q.len + k - 1u) / k;
+    return q;
+}
+
+// The item of number `item`; false if there is none. All 64 lanes take part,
+// and every wave of the grid gets the same plan.
+__device__ bool paged_item(const PagedAttnParams& p, uint32_t item, PagedItem* it) {
+    const uint32_t lane = threadIdx.x & (kWave - 1);
+    const uint32_t seqs = p.g.seqs;
+    const PagedSeqPlan q0 = paged_seq_plan(p, lane);
+    auto cost_of = [&](const PagedSeqPlan& q) {
+        return (float)q.tiles * (float)q.steps * (q.narrow ? p.narrow_cost : p.wide_cost);
+    };
+    float total = wave_sum(cost_of(q0));
+    for (uint32_t b = kWave; b < seqs; b += kWave) total += wave_sum(cost_of(paged_seq_plan(p, b + lane)));
+    const float share = fmaxf(total * (float)p.g.KVH / p.target, p.least);
+    uint64_t base = 0;
+    for (uint32_t b = 0; b < seqs; b += kWave) {
+        const PagedSeqPlan q = b == 0 ? q0 : paged_seq_plan(p, b + lane);
+        const float per_f = ceilf(share / (q.narrow ? p.narrow_cost : p.wide_cost));
+        const uint32_t per = (uint32_t)fminf(fmaxf(per_f, 1.f), 1e9f);
+        const uint32_t chunks = max((q.steps + per - 1u) / per, 1u);
+        const uint64_t mine = (uint64_t)p.g.KVH * q.tiles * chunks;
+        uint64_t sum = mine;                                  // inclusive scan
+#pragma unroll
+        for (int o = 1; o < kWave; o <<= 1) {
+            const uint64_t v = __shfl_up((unsigned long long)sum, o, kWave);
+            if (lane >= (uint32_t)o) sum += v;
+        }
+        const uint64_t end = base + sum, begin = end - mine;
+        const uint64_t hit = __ballot(item >= begin && item < end);
+        if (hit) {
+            const int w = __builtin_ctzll(hit);
+            auto u = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, w); };
+            const uint64_t b0 = (uint64_t)u((uint32_t)begin) | ((uint64_t)u((uint32_t)(begin >> 32)) << 32);
+            const uint64_t e0 = (uint64_t)u((uint32_t)end) | ((uint64_t)u((uint32_t)(end >> 32)) << 32);
+            // row offsets that are none can ask for more items than the grid has: all of such a sequence is left out
+            if (e0 > gridDim.x) return false;
+            it->s = b + (uint32_t)w;
+            it->tiles = u(q.tiles);
+            it->chunks = u(chunks);
+            it->per = u(per);
+            it->row0 = u(q.row0);
+            it->n = u(q.n);
+            it->len = u(q.len);
+            it->pos0 = (int64_t)((uint64_t)u((uint32_t)(uint64_t)q.pos0) | ((uint64_t)u((uint32_t)((uint64_t)q.pos0 >> 32)) << 32));
+            it->narrow = u(q.narrow ? 1u : 0u) != 0u;
+            // KV head fastest (a head's items keep to the same XCDs' L2), then the tiles that share a chunk of keys
+            uint32_t r = item - (uint32_t)b0;
+            it->kvh = r % p.g.KVH;
+            r /= p.g.KVH;
+            it->tile = r % it->tiles;
+            it->chunk = r / it->tiles;
+            it->first = (uint32_t)b0 + it->tile * p.g.KVH + it->kvh;
+            return true;
+        }
+        base += (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)sum, kWave - 1) |
+                ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(sum >> 32), kWave - 1) << 32);
+        if (base > item) return false;
+    }
+    return false;
+}
+
+// Where a key's row starts, in units of 16 bytes from the pool's first byte
+// (32 bits reach 64 GB), and whether it is there.
+__device__ __forceinline__ uint32_t paged_row_unit(const PagedAttnParams& p, uint32_t kvh, int32_t page, uint32_t slot) {
+    return (uint32_t)page * p.page_u + kvh * p.head_u + slot * p.slot_u;
+}
+
+// x = hi + lo in binary16 for two values: hi cut (v_cvt_pkrtz), lo the rounded rest.
+__device__ __forceinline__ void pg_split2(float a, float b, uint32_t* hi, uint32_t* lo) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+    *hi = __builtin_bit_cast(uint32_t, h);
+    const half2v r = {(_Float16)(a - (float)h[0]), (_Float16)(b - (float)h[1])};
+    *lo = __builtin_bit_cast(uint32_t, r);
+}
+
+// Three bfloat16 parts of two values, packed (a low, b high): cutting 8 bits at a time is exact.
+__device__ __forceinline__ void pg_cut2(float a, float b, uint32_t* p1, uint32_t* p2, uint32_t* p3) {
+    const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+    *p1 = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
+    const float a2 = a - __uint_as_float(ua & 0xFFFF0000u), b2 = b - __uint_as_float(ub & 0xFFFF0000u);
+    const uint32_t va = __float_as_uint(a2), vb = __float_as_uint(b2);
+    *p2 = __builtin_amdgcn_perm(vb, va, 0x07060302u);
+    const float a3 = a2 - __uint_as_float(va & 0xFFFF0000u), b3 = b2 - __uint_as_float(vb & 0xFFFF0000u);
+    *p3 = __builtin_amdgcn_perm(__float_as_uint(b3), __float_as_uint(a3), 0x07060302u);
+}
+
+// The last of a tile's chunks to arrive joins their states: every chunk's state is stored past this
+// XCD's L2 (agent scope) before its arrival is counted; the counter is zero again afterwards.
+__device__ __forceinline__ bool paged_arrive(uint32_t* count, uint32_t live, uint32_t* shared) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // this wave's state is in place
     __syncthreads();
-    float m = -INFINITY, l = 0.f, o[2] = {0.f, 0.f};
-    for (uint32_t k0 = 0; k0 < nk; k0 += kWave) {
-        uint32_t entry = 0, slot = 0;
-        bool on = k0 + lane < nk && paged_table_index(k0 + lane, g.page_size, g.max_pages, &entry, &slot);
-        uint64_t at = 0;
-        float sc = -INFINITY;
-        if (on) {
-            const int32_t page = g.pages[(uint64_t)s * g.max_pages + entry];
-            on = paged_page_ok(page, g.num_pages);
-            if (on) {
-                at = paged_offset(g.page_stride, g.head_stride, g.slot_stride, (uint32_t)page, h / p.G, slot);
-                float dot = 0.f;
-                for (uint32_t d = 0; d < g.hd; ++d) {
-                    const float kv = F16KV ? h2f(reinterpret_cast<const uint16_t*>(g.k)[at + d])
-                                           : reinterpret_cast<const float*>(g.k)[at + d];
-                    dot = fmaf(qs[d], kv, dot);
+    if (threadIdx.x == 0) {
+        const uint32_t n = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (n == live - 1u) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *shared = n;
+    }
+    __syncthreads();
+    return *shared == live - 1u;
+}
+
+using pg_u64 = unsigned long long;
+__device__ __forceinline__ void pg_put2(float* p, float a, float b) {
+    const pg_u64 v = (pg_u64)__float_as_uint(a) | ((pg_u64)__float_as_uint(b) << 32);
+    __hip_atomic_store(reinterpret_cast<pg_u64*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 pg_get2(const float* p) {
+    const pg_u64 v = __hip_atomic_load(reinterpret_cast<const pg_u64*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+
+// Binary16 words / float32 words that are infinite or NaN.
+template <bool F16>
+__device__ __forceinline__ bool pg_not_finite(uint32_t w) {
+    if constexpr (F16) return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u;
+    else return (w & 0x7F800000u) == 0x7F800000u;
+}
+
+// One value of the pool, as float.
+template <bool F16>
+__device__ __forceinline__ float pg_value(const void* pool, uint32_t unit, uint32_t d) {
+    const char* b = reinterpret_cast<const char*>(pool) + ((uint64_t)unit << 4);
+    if constexpr (F16) return h2f(reinterpret_cast<const uint16_t*>(b)[d]);
+    else return reinterpret_cast<const float*>(b)[d];
+}
+
+// ---- narrow items ----
+// Wave w takes keys NK (4 i + w) .. of the chunk, NK = 32 (float32: 16) a step.
+// Lane (g, li) = (l / 16, l % 16): the scores of row li for keys 16 c + 4 g + r
+// (v_mfma_f32_16x16x32: A = K rows, B = q rows), so V^T P^T needs V of those
+// keys in lane group g: the lane loads dims HD / 16 li .. of each and pairs the keys up with
+// v_perm (32 for 32 keys x 128 dims, no LDS). K of the next step goes out once the scores have
+// used K's registers, V's likewise; page ids are read two steps ahead.
+template <int HD, bool F16>
+__device__ __forceinline__ void paged_narrow(const PagedAttnParams& p, const PagedItem& it, float* red, uint32_t* shared) {
+    constexpr uint32_t NK = pg_narrow_keys(F16) / 4u;
+    constexpr int KC = NK / 16;                              // 16-key score tiles
+    constexpr int QC = HD / 32;                              // 32-deep steps of q.k
+    constexpr int DL = HD / 16;                              // dims of V a lane holds
+    constexpr int NP = F16 ? 2 : 3;                          // parts of q and the weights
+    constexpr uint32_t ES = F16 ? 2u : 4u;
+    constexpr int VR = 4 * KC;                               // V rows of a lane
+    constexpr int VW = DL * (int)ES / 4;                     // words of one
+    const PagedParams& g = p.g;
+    const uint32_t t = threadIdx.x, lane = t % kWave, g4 = lane / 16u, li = lane % 16u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(t / kWave);
+    const uint32_t M = it.n * p.G, hd = g.hd;
+    const uint32_t kbeg = it.chunk * it.per * (4u * NK);
+    const uint32_t kend = min(it.len, kbeg + it.per * (4u * NK));
+    const uint32_t rr = min(li, M - 1u), tok = rr / p.G, head = it.kvh * p.G + rr % p.G;
+    const float* qrow = p.q + (uint64_t)(it.row0 + tok) * p.ldq + (uint64_t)head * hd;
+    const int32_t* table = g.pages + (uint64_t)it.s * g.max_pages;
+    const char* kpool = reinterpret_cast<const char*>(g.k);
+    const char* vpool = reinterpret_cast<const char*>(g.v);
+    const uint32_t kl = lane % NK;                           // the key whose place this lane looks up
+
+    auto page_of = [&](uint32_t k0) {                        // (past the end: some entry that is not used)
+        return table[min(k0 + kl, max(kend, 1u) - 1u) / g.page_size];
+    };
+    // the lane's key's row (pool row 0 where it is not there), and which keys are
+    auto unit_of = [&](uint32_t k0, int32_t page, uint32_t* live) {
+        const uint32_t key = k0 + kl;
+        const bool on = key < kend && paged_page_ok(page, g.num_pages);
+        *live = (uint32_t)(__ballot(on) & ((1ull << NK) - 1ull));
+        return on ? paged_row_unit(p, it.kvh, page, key % g.page_size) : it.kvh * p.head_u;
+    };
+    auto row_at = [&](uint32_t unit, uint32_t key) {
+        return (uint64_t)(uint32_t)__builtin_amdgcn_ds_bpermute((int)(4u * key), (int)unit) << 4;
+    };
+    constexpr int KW = F16 ? 1 : 2;                          // 16-byte loads of 8 dims
+    v4u32 kr[KC][QC][KW];
+    uint32_t vr[VR][VW];
+    auto load_k = [&](uint32_t unit) {
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            const char* b = kpool + row_at(unit, 16u * c + li);
+#pragma unroll
+            for (int st = 0; st < QC; ++st) {
+                const uint32_t d = 32u * st + 8u * g4;
+                const char* a = b + (d < hd ? d : 0u) * ES;   // (dims past hd: q is zero there)
+#pragma unroll
+                for (int w = 0; w < KW; ++w) kr[c][st][w] = ld_global<v4u32>(a + 16 * w);
+            }
+        }
+    };
+    auto load_v = [&](uint32_t unit) {
+        const uint32_t d = li * DL < hd ? li * DL : 0u;
+#pragma unroll
+        for (int b = 0; b < VR; ++b) {
+            const char* a = vpool + row_at(unit, 16u * (b / 4) + 4u * g4 + b % 4) + d * ES;
+            if constexpr (VW == 2) {
+                const v2u32 x = ld_global<v2u32>(a);
+                vr[b][0] = x[0];
+                vr[b][1] = x[1];
+            } else {
+#pragma unroll
+                for (int w = 0; w < VW / 4; ++w) {
+                    const v4u32 x = ld_global<v4u32>(a + 16 * w);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) vr[b][4 * w + i] = x[i];
                 }
-                sc = dot * p.scale;
             }
         }
-        const float mn = fmaxf(m, wave_max(sc));
+    };
+
+    uint32_t k0 = kbeg + wave * NK;
+    int32_t page = page_of(k0), page1 = page_of(k0 + 4u * NK);
+    float qv[QC][8];
+#pragma unroll
+    for (int st = 0; st < QC; ++st) {
+        const uint32_t d = 32u * st + 8u * g4;
+        const float4 a = *reinterpret_cast<const float4*>(qrow + (d < hd ? d : 0u));
+        const float4 b = *reinterpret_cast<const float4*>(qrow + (d < hd ? d : 0u) + 4);
+        const bool in = d < hd;
+        qv[st][0] = in ? a.x : 0.f; qv[st][1] = in ? a.y : 0.f; qv[st][2] = in ? a.z : 0.f; qv[st][3] = in ? a.w : 0.f;
+        qv[st][4] = in ? b.x : 0.f; qv[st][5] = in ? b.y : 0.f; qv[st][6] = in ? b.z : 0.f; qv[st][7] = in ? b.w : 0.f;
+    }
+    uint32_t live, live1;
+    uint32_t unit = unit_of(k0, page, &live);
+    load_k(unit);
+    load_v(unit);
+    v4u32 qp[NP][QC];
+    float qf = p.scale * 1.4426950408889634f;                // scores in log2 units
+    {
+        float amax = 0.f;
+#pragma unroll
+        for (int st = 0; st < QC; ++st)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(qv[st][i]));
+        int e = 0;
+        if constexpr (F16) {
+            (void)frexpf(max_row_slots(amax), &e);
+            e -= 15;
+            qf *= ldexpf(1.f, e);
+        }
+#pragma unroll
+        for (int st = 0; st < QC; ++st)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t w[3];
+                if constexpr (F16) pg_split2(ldexpf(qv[st][2 * i], -e), ldexpf(qv[st][2 * i + 1], -e), &w[0], &w[1]);
+                else pg_cut2(qv[st][2 * i], qv[st][2 * i + 1], &w[0], &w[1], &w[2]);
+#pragma unroll
+                for (int a = 0; a < NP; ++a) qp[a][st][i] = w[a];
+            }
+    }
+    const int64_t qpos64 = it.pos0 + (int64_t)tok;
+    const int32_t qpos = (int32_t)max((int64_t)-1, min(qpos64, (int64_t)0x7FFFFFFF));
+    constexpr float kBoost = F16 ? 15.f : 0.f;               // weights times 2^15 (binary16's range)
+    float m = -INFINITY, l = 0.f;
+    pg_f4 o[DL];
+#pragma unroll
+    for (int e = 0; e < DL; ++e) o[e] = pg_f4{0.f, 0.f, 0.f, 0.f};
+
+    for (; k0 < kend; k0 += 4u * NK) {
+        const int32_t page2 = page_of(k0 + 8u * NK);
+        // ---- scores ----
+        pg_f4 sacc[KC];
+#pragma unroll
+        for (int c = 0; c < KC; ++c) sacc[c] = pg_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < QC; ++st) {
+            if constexpr (F16) {
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int c = 0; c < KC; ++c)
+                        sacc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pg_half8, kr[c][st][0]),
+                                                                         __builtin_bit_cast(pg_half8, qp[a][st]), sacc[c], 0, 0, 0);
+            } else {
+                v4u32 kp[3];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t w[3];
+                    const v4u32 x = kr[0][st][i / 2];
+                    pg_cut2(__uint_as_float(x[2 * (i % 2)]), __uint_as_float(x[2 * (i % 2) + 1]), &w[0], &w[1], &w[2]);
+#pragma unroll
+                    for (int a = 0; a < 3; ++a) kp[a][i] = w[a];
+                }
+#pragma unroll
+                for (int a = 2; a >= 0; --a)
+#pragma unroll
+                    for (int b = 2 - a; b >= 0; --b)
+                        sacc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pg_bf8, kp[a]),
+                                                                          __builtin_bit_cast(pg_bf8, qp[b][st]), sacc[0], 0, 0, 0);
+            }
+        }
+        const uint32_t k1 = k0 + 4u * NK;
+        const uint32_t unit1 = unit_of(k1, page1, &live1);
+        load_k(unit1);
+        // ---- masks: keys that are not there, and rows before a key ----
+        const uint32_t all = (uint32_t)((1ull << NK) - 1ull);
+        const bool full = live == all && (int64_t)(k0 + NK - 1u) <= it.pos0;
+        float sv[KC][4];
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sv[c][r] = sacc[c][r] * qf;
+        if (!full) {
+#pragma unroll
+            for (int c = 0; c < KC; ++c)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint32_t key = 16u * c + 4u * g4 + r;
+                    if (!((live >> key) & 1u) || (int32_t)(k0 + key) > qpos) sv[c][r] = -INFINITY;
+                }
+        }
+        // ---- running softmax of row li ----
+        float mx = sv[0][0];
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sv[c][r]);
+        mx = max_row_slots(mx);
+        const float mn = fmaxf(m, mx);
         const float mref = mn == -INFINITY ? 0.f : mn;
-        const float f = expf(m - mref), e = on ? expf(sc - mref) : 0.f;
-        l = l * f + wave_sum(e);
-        m = mn;
-        const uint64_t live = __ballot(on);
-        __syncthreads();
-        es[lane] = e;
-        offs[lane] = at;
-        __syncthreads();
-        o[0] *= f;
-        o[1] *= f;
-        for (uint32_t j = 0; j < (uint32_t)kWave; ++j) {
-            if (!((live >> j) & 1u)) continue;
+        if (__ballot(mn > m)) {
+            const float f = __builtin_amdgcn_exp2f(m - mref);
+            l *= f;
 #pragma unroll
-            for (uint32_t i = 0; i < 2; ++i) {
-                const uint32_t d = lane + kWave * i;
-                if (d >= g.hd) continue;
-                const float v = F16KV ? h2f(reinterpret_cast<const uint16_t*>(g.v)[offs[j] + d])
-                                      : reinterpret_cast<const float*>(g.v)[offs[j] + d];
-                o[i] = fmaf(es[j], v, o[i]);
+            for (int e = 0; e < DL; ++e)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[e][r] *= f;
+        }
+        m = mn;
+        float ev[KC][4];
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                ev[c][r] = __builtin_amdgcn_exp2f(sv[c][r] - mref + kBoost);
+                l += ev[c][r];
+            }
+        // ---- values: rows nobody sees read as zero; a row that only some see must not
+        // meet the others' zero weights when it is not finite ----
+        if (!full) {
+            uint32_t bad = 0;
+#pragma unroll
+            for (int b = 0; b < VR; ++b) {
+                const uint32_t key = 16u * (b / 4) + 4u * g4 + b % 4;
+                const bool on = (live >> key) & 1u;
+                bool nf = false;
+#pragma unroll
+                for (int w = 0; w < VW; ++w) {
+                    vr[b][w] = on ? vr[b][w] : 0u;
+                    nf = nf || pg_not_finite<F16>(vr[b][w]);
+                }
+                // (a lane past hd holds dims 0 ..: the same row)
+                const uint64_t who = __ballot(nf && (int64_t)(k0 + key) > it.pos0);
+#pragma unroll
+                for (int gg = 0; gg < 4; ++gg)
+                    if ((who >> (16 * gg)) & 0xFFFFull) bad |= 1u << (16 * (b / 4) + 4 * gg + b % 4);
+            }
+            if (bad) {
+#pragma unroll
+                for (int b = 0; b < VR; ++b)
+                    if ((bad >> (16u * (b / 4) + 4u * g4 + b % 4)) & 1u)
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) vr[b][w] = 0u;
+                for (uint32_t rest = bad; rest; rest &= rest - 1u) {
+                    const uint32_t key = (uint32_t)__builtin_ctz(rest);
+                    float mine = 0.f;
+#pragma unroll
+                    for (int c = 0; c < KC; ++c)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) mine = (uint32_t)(4 * c + r) == 4u * (key / 16u) + key % 4u ? ev[c][r] : mine;
+                    const float w = __shfl(mine, (int)(16u * ((key % 16u) / 4u) + li), kWave);
+                    const uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)unit, (int)key);
+                    if ((int32_t)(k0 + key) <= qpos) {
+#pragma unroll
+                        for (int e = 0; e < DL; ++e)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const uint32_t d = DL * (4u * g4 + r) + e;
+                                if (d < hd) o[e][r] = fmaf(w, pg_value<F16>(g.v, at, d), o[e][r]);
+                            }
+                    }
+                }
+            }
+        }
+        // ---- O^T += V^T P^T ----
+        if constexpr (F16) {
+            v4u32 pp[2];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t h, w;
+                pg_split2(ev[i / 2][2 * (i % 2)], ev[i / 2][2 * (i % 2) + 1], &h, &w);
+                pp[0][i] = h;
+                pp[1][i] = w;
+            }
+#pragma unroll
+            for (int e2 = 0; e2 < DL / 2; ++e2) {
+                v4u32 v0, v1;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v0[i] = __builtin_amdgcn_perm(vr[2 * i + 1][e2], vr[2 * i][e2], 0x05040100u);
+                    v1[i] = __builtin_amdgcn_perm(vr[2 * i + 1][e2], vr[2 * i][e2], 0x07060302u);
+                }
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    const pg_half8 pb = __builtin_bit_cast(pg_half8, pp[a]);
+                    o[2 * e2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pg_half8, v0), pb, o[2 * e2], 0, 0, 0);
+                    o[2 * e2 + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pg_half8, v1), pb, o[2 * e2 + 1], 0, 0, 0);
+                }
+            }
+        } else {
+            v2u32 pp[3];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                uint32_t w[3];
+                pg_cut2(ev[0][2 * i], ev[0][2 * i + 1], &w[0], &w[1], &w[2]);
+#pragma unroll
+                for (int a = 0; a < 3; ++a) pp[a][i] = w[a];
+            }
+#pragma unroll
+            for (int e = 0; e < DL; ++e) {
+                v2u32 vp[3];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t w[3];
+                    pg_cut2(__uint_as_float(vr[2 * i][e]), __uint_as_float(vr[2 * i + 1][e]), &w[0], &w[1], &w[2]);
+#pragma unroll
+                    for (int a = 0; a < 3; ++a) vp[a][i] = w[a];
+                }
+#pragma unroll
+                for (int a = 2; a >= 0; --a)
+#pragma unroll
+                    for (int b = 2 - a; b >= 0; --b)
+                        o[e] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(pg_s4, vp[a]),
+                                                                         __builtin_bit_cast(pg_s4, pp[b]), o[e], 0, 0, 0);
+            }
+        }
+        load_v(unit1);
+        unit = unit1;
+        live = live1;
+        page1 = page2;
+    }
+
+    // ---- the four waves' states: thread = row t / 16, dims DL (t % 16) .. ----
+    constexpr uint32_t LD = HD + 4;                          // padded LDS row
+    float* rm = red + 4u * 16u * LD;                         // [wave][row] m, then l
+    l = sum_row_slots(l);
+#pragma unroll
+    for (int e = 0; e < DL; ++e)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) red[(wave * 16u + li) * LD + DL * (4u * g4 + r) + e] = o[e][r];
+    if (g4 == 0) {
+        rm[wave * 16u + li] = m;
+        rm[64u + wave * 16u + li] = l;
+    }
+    __syncthreads();
+    const uint32_t row = t / 16u, d0 = DL * (t % 16u);
+    float M0 = -INFINITY, L0 = 0.f, acc[DL];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) M0 = fmaxf(M0, rm[w * 16u + row]);
+    const float mr = M0 == -INFINITY ? 0.f : M0;
+#pragma unroll
+    for (int d = 0; d < DL; ++d) acc[d] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float f = __builtin_amdgcn_exp2f(rm[w * 16u + row] - mr);
+        L0 = fmaf(f, rm[64u + w * 16u + row], L0);
+#pragma unroll
+        for (int d = 0; d < DL; ++d) acc[d] = fmaf(f, red[(w * 16u + row) * LD + d0 + d], acc[d]);
+    }
+    if (it.chunks > 1u) {
+        const uint32_t stride = it.tiles * g.KVH;            // items of a tile's neighbouring chunks
+        auto state = [&](uint32_t c) { return p.part + (uint64_t)(it.first + c * stride) * p.part_floats; };
+        if (row < M) {
+            float* d = state(it.chunk);
+#pragma unroll
+            for (int i = 0; i < DL; i += 2) pg_put2(d + row * HD + d0 + i, acc[i], acc[i + 1]);
+            if (t % 16u == 0) pg_put2(d + 16u * HD + 2u * row, M0, L0);
+        }
+        if (!paged_arrive(p.count + it.first, it.chunks, shared)) return;
+        if (row >= M) return;
+        float mx = -INFINITY;
+        for (uint32_t c = 0; c < it.chunks; ++c) mx = fmaxf(mx, pg_get2(state(c) + 16u * HD + 2u * row).x);
+        const float mf = mx == -INFINITY ? 0.f : mx;
+        L0 = 0.f;
+#pragma unroll
+        for (int d = 0; d < DL; ++d) acc[d] = 0.f;
+#pragma unroll 4
+        for (uint32_t c = 0; c < it.chunks; ++c) {
+            const float* b = state(c);
+            const float2 ml = pg_get2(b + 16u * HD + 2u * row);
+            float2 x[DL / 2];
+#pragma unroll
+            for (int i = 0; i < DL / 2; ++i) x[i] = pg_get2(b + row * HD + d0 + 2 * i);
+            const float f = __builtin_amdgcn_exp2f(ml.x - mf);
+            L0 = fmaf(f, ml.y, L0);
+#pragma unroll
+            for (int i = 0; i < DL / 2; ++i) {
+                acc[2 * i] = fmaf(f, x[i].x, acc[2 * i]);
+                acc[2 * i + 1] = fmaf(f, x[i].y, acc[2 * i + 1]);
             }
         }
     }
-    const float inv = nk && m > -INFINITY ? 1.0f / l : (m == m ? 0.f : m);
+    if (row >= M || d0 >= hd) return;
+    const float inv = L0 == 0.f ? 0.f : 1.0f / L0;           // a row that sees nothing: zeros
+    float* out = p.out + (uint64_t)(it.row0 + row / p.G) * p.ldo + (uint64_t)(it.kvh * p.G + row % p.G) * hd + d0;
 #pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) {
-        const uint32_t d = lane + kWave * i;
-        if (d < g.hd) p.out[(uint64_t)row * p.ldo + (uint64_t)h * g.hd + d] = o[i] * inv;
+    for (int i = 0; i < DL; i += 4)
+        *reinterpret_cast<float4*>(out + i) = make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
+}
+
+// ---- wide items ----
+// Wave w holds rows 32 w .. of the tile as columns of 32 x 32 products: S^T = K Q^T
+// (v_mfma_f32_32x32x16), lane (h, c) = (l / 32, l % 32) with row c's scores of keys
+// 8 j + 4 h + r, then O^T += V^T P^T with V^T from transposing LDS reads
+// (ds_read_b64_tr_b16: 4 keys x 16 dims of a row-major tile). Over a binary16 cache the tile
+// goes from the cache to LDS past the registers, one tile ahead, two buffers and one barrier
+// a tile; a float32 tile is loaded into registers a tile ahead and cut into its three parts
+// on the way to LDS. 16-byte pieces of an LDS row are permuted by the row so that neither the
+// reads of 32 keys' pieces nor the transposing reads of 4 keys meet in a bank.
+// What bounds a chunk of 512 rows over 8192 keys is the matrix cores' two (six) products and
+// the softmax's vector instructions beside them, about as many cycles.
+template <int HD>
+__device__ __forceinline__ uint32_t pg_swz_k(uint32_t row) {
+    return HD == 128 ? row & 15u : (row >> 1) & 7u;
+}
+template <int HD>
+__device__ __forceinline__ uint32_t pg_swz_v(uint32_t row) {
+    return HD == 128 ? ((row & 3u) << 2) | ((row >> 2) & 3u) : (((row >> 1) & 1u) << 2) | ((row >> 2) & 3u);
+}
+
+template <int HD, bool F16>
+__device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const PagedItem& it, char* smem, uint32_t* shared) {
+    constexpr uint32_t KT = pg_wide_keys(F16);
+    constexpr int KB = KT / 32;                              // 32-key score tiles
+    constexpr int QS = HD / 16;                              // 16-deep steps of q.k
+    constexpr int OD = HD / 32;                              // 32-dim output tiles
+    constexpr int NP = F16 ? 2 : 3;                          // parts of q and the weights
+    constexpr int KP = F16 ? 1 : 3;                          // parts of k and v
+    constexpr uint32_t ES = F16 ? 2u : 4u;
+    constexpr uint32_t CPR = HD / 8;                         // 16-byte pieces of an LDS row
+    constexpr uint32_t TB = KT * HD * 2u;                    // bytes of a tile part in LDS
+    const PagedParams& g = p.g;
+    const uint32_t t = threadIdx.x, lane = t % kWave, h = lane / 32u, li = lane % 32u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(t / kWave);
+    const uint64_t M = (uint64_t)it.n * p.G;
+    const uint32_t hd = g.hd;
+    const uint32_t r0 = it.tile * kPgWideRows;               // first flattened row of the tile
+    const uint32_t nrow = (uint32_t)min((uint64_t)kPgWideRows, M - r0);
+    // keys that the tile's last row sees bound its chunks
+    const int64_t last_pos = it.pos0 + (int64_t)((r0 + nrow - 1u) / p.G);
+    const uint32_t klen = (uint32_t)max((int64_t)0, min((int64_t)it.len, last_pos + 1));
+    const uint32_t ckeys = it.per > 0x7FFFFFFFu / KT ? 0x7FFFFFFFu / KT * KT : it.per * KT;
+    const uint32_t lives = max(1u, (klen + ckeys - 1u) / ckeys);
+    if (it.chunk >= lives) return;
+    const uint32_t kbeg = it.chunk * ckeys, kend = min(klen, kbeg + ckeys);
+    const bool wave_on = wave * 32u < nrow;
+    const uint32_t rr = r0 + min(wave * 32u + li, nrow - 1u);
+    const uint32_t tok = rr / p.G, head = it.kvh * p.G + rr % p.G;
+    const float* qrow = p.q + (uint64_t)(it.row0 + tok) * p.ldq + (uint64_t)head * hd;
+    const int32_t* table = g.pages + (uint64_t)it.s * g.max_pages;
+    const int64_t first_pos = it.pos0 + (int64_t)((r0 + min(wave * 32u, nrow - 1u)) / p.G);   // of the wave's rows
+    const int32_t qpos = (int32_t)max((int64_t)-1, min(it.pos0 + (int64_t)tok, (int64_t)0x7FFFFFFF));
+
+    const uint32_t kl = lane % KT;
+    auto page_of = [&](uint32_t k0) { return table[min(k0 + kl, max(kend, 1u) - 1u) / g.page_size]; };
+    auto unit_of = [&](uint32_t k0, int32_t page, uint64_t* live) {
+        const uint32_t key = k0 + kl;
+        const bool on = key < kend && paged_page_ok(page, g.num_pages);
+        *live = __ballot(on) & (KT == 64u ? ~0ull : (1ull << (KT % 64u)) - 1ull);
+        return on ? paged_row_unit(p, it.kvh, page, key % g.page_size) : it.kvh * p.head_u;
+    };
+    auto row_at = [&](uint32_t unit, uint32_t key) {
+        return (uint64_t)(uint32_t)__builtin_amdgcn_ds_bpermute((int)(4u * key), (int)unit) << 4;
+    };
+    char* const kt0 = smem;                                  // binary16: [buffer]; float32: [part]
+    char* const vt0 = smem + (F16 ? 2u : 3u) * TB;
+    constexpr int NL = (int)(KT * HD * ES / 16u / 256u);     // 16-byte pieces of K (and V) a thread moves
+    v4u32 kreg[F16 ? 1 : NL], vreg[F16 ? 1 : NL];
+    auto load_tile = [&](uint32_t unit, uint32_t buf) {
+#pragma unroll
+        for (int j = 0; j < NL; ++j) {
+            const uint32_t n = (wave * NL + (uint32_t)j) * kWave + lane;
+            if constexpr (F16) {
+                // piece n of the tile: LDS takes a wave's pieces in lane order
+                const uint32_t row = n / CPR, c = n % CPR, ck = c ^ pg_swz_k<HD>(row), cv = c ^ pg_swz_v<HD>(row);
+                const uint64_t at = row_at(unit, row);
+                const char* ks = reinterpret_cast<const char*>(g.k) + at + (8u * ck < hd ? ck : 0u) * 16u;
+                const char* vs = reinterpret_cast<const char*>(g.v) + at + (8u * cv < hd ? cv : 0u) * 16u;
+                char* kd = kt0 + buf * TB + (wave * NL + (uint32_t)j) * 1024u;
+                char* vd = vt0 + buf * TB + (wave * NL + (uint32_t)j) * 1024u;
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(uint64_t)ks,
+                                                 (__attribute__((address_space(3))) void*)kd, 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(uint64_t)vs,
+                                                 (__attribute__((address_space(3))) void*)vd, 16, 0, 0);
+            } else {
+                const uint32_t row = n / (HD / 4), c = n % (HD / 4);
+                const uint64_t at = row_at(unit, row) + (4u * c < hd ? c : 0u) * 16u;
+                kreg[j] = ld_global<v4u32>(reinterpret_cast<const char*>(g.k) + at);
+                vreg[j] = ld_global<v4u32>(reinterpret_cast<const char*>(g.v) + at);
+            }
+        }
+    };
+    auto store_tile = [&]() {                                // float32: three parts of four dims, 8 bytes each
+        if constexpr (!F16) {
+#pragma unroll
+            for (int j = 0; j < NL; ++j) {
+                const uint32_t n = (wave * NL + (uint32_t)j) * kWave + lane;
+                const uint32_t row = n / (HD / 4), c = n % (HD / 4);
+                const uint32_t ak = (row * CPR + ((c / 2u) ^ pg_swz_k<HD>(row))) * 16u + (c % 2u) * 8u;
+                const uint32_t av = (row * CPR + ((c / 2u) ^ pg_swz_v<HD>(row))) * 16u + (c % 2u) * 8u;
+                uint32_t a[3], b[3];
+                pg_cut2(__uint_as_float(kreg[j][0]), __uint_as_float(kreg[j][1]), &a[0], &a[1], &a[2]);
+                pg_cut2(__uint_as_float(kreg[j][2]), __uint_as_float(kreg[j][3]), &b[0], &b[1], &b[2]);
+#pragma unroll
+                for (uint32_t q = 0; q < 3; ++q) *reinterpret_cast<uint2*>(kt0 + q * TB + ak) = make_uint2(a[q], b[q]);
+                pg_cut2(__uint_as_float(vreg[j][0]), __uint_as_float(vreg[j][1]), &a[0], &a[1], &a[2]);
+                pg_cut2(__uint_as_float(vreg[j][2]), __uint_as_float(vreg[j][3]), &b[0], &b[1], &b[2]);
+#pragma unroll
+                for (uint32_t q = 0; q < 3; ++q) *reinterpret_cast<uint2*>(vt0 + q * TB + av) = make_uint2(a[q], b[q]);
+            }
+        }
+    };
+
+    int32_t page = page_of(kbeg), page1 = page_of(kbeg + KT);
+    v4u32 qp[NP][QS];
+    float qf = p.scale * 1.4426950408889634f;
+    {
+        float qv[QS][8], amax = 0.f;
+#pragma unroll
+        for (int st = 0; st < QS; ++st) {
+            const uint32_t d = 16u * st + 8u * h;
+            const bool in = d < hd;
+            const float4 a = *reinterpret_cast<const float4*>(qrow + (in ? d : 0u));
+            const float4 b = *reinterpret_cast<const float4*>(qrow + (in ? d : 0u) + 4);
+            qv[st][0] = in ? a.x : 0.f; qv[st][1] = in ? a.y : 0.f; qv[st][2] = in ? a.z : 0.f; qv[st][3] = in ? a.w : 0.f;
+            qv[st][4] = in ? b.x : 0.f; qv[st][5] = in ? b.y : 0.f; qv[st][6] = in ? b.z : 0.f; qv[st][7] = in ? b.w : 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(qv[st][i]));
+        }
+        int e = 0;
+        if constexpr (F16) {
+            amax = fmaxf(amax, __shfl_xor(amax, 32, kWave));
+            (void)frexpf(amax, &e);
+            e -= 15;
+            qf *= ldexpf(1.f, e);
+        }
+#pragma unroll
+        for (int st = 0; st < QS; ++st)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t w[3];
+                if constexpr (F16) pg_split2(ldexpf(qv[st][2 * i], -e), ldexpf(qv[st][2 * i + 1], -e), &w[0], &w[1]);
+                else pg_cut2(qv[st][2 * i], qv[st][2 * i + 1], &w[0], &w[1], &w[2]);
+#pragma unroll
+                for (int a = 0; a < NP; ++a) qp[a][st][i] = w[a];
+            }
     }
+    constexpr float kBoost = F16 ? 15.f : 0.f;
+    float m = -INFINITY, l = 0.f;
+    pg_f16 o[OD];
+#pragma unroll
+    for (int d = 0; d < OD; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[d][v] = 0.f;
+
+    uint64_t live, live1 = 0;
+    uint32_t unit = unit_of(kbeg, page, &live);
+    load_tile(unit, 0);
+    uint32_t buf = 0;
+    // V^T piece of dim tile d, 16 keys 16 t4 .., part q: the lane's dim, keys 8 j + 4 h + r
+    const uint32_t l16 = lane % 16u, vrow = 4u * h + l16 / 4u;
+    auto v_frag = [&](const char* vt, int t4, int d) {
+        v4u32 a;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t row = 16u * t4 + 8u * j + vrow;
+            const uint32_t c = 4u * d + 2u * ((lane / 16u) % 2u) + (l16 % 4u) / 2u;
+            const char* at = vt + (row * CPR + (c ^ pg_swz_v<HD>(row))) * 16u + (l16 % 2u) * 8u;
+            const v2u32 x = __builtin_bit_cast(v2u32, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                          (__attribute__((address_space(3))) pg_s4*)at));
+            a[2 * j] = x[0];
+            a[2 * j + 1] = x[1];
+        }
+        return a;
+    };
+    for (uint32_t k0 = kbeg; k0 < kend; k0 += KT) {
+        if constexpr (!F16) {
+            __syncthreads();                                 // the previous tile is consumed
+            store_tile();
+        }
+        __syncthreads();                                     // (waits for this wave's loads to LDS first)
+        const int32_t page2 = page_of(k0 + 2u * KT);
+        const uint32_t unit1 = unit_of(k0 + KT, page1, &live1);
+        if (k0 + KT < kend) load_tile(unit1, buf ^ 1u);
+        const char* kt = kt0 + (F16 ? buf * TB : 0u);
+        const char* vt = vt0 + (F16 ? buf * TB : 0u);
+        const uint64_t live_now = live;
+        const uint32_t unit_now = unit;
+        buf ^= 1u;
+        unit = unit1;
+        live = live1;
+        page1 = page2;
+        if (!wave_on) continue;
+        // ---- scores ----
+        pg_f16 sacc[KB];
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) sacc[b][v] = 0.f;
+#pragma unroll
+        for (int st = 0; st < QS; ++st) {
+            v4u32 kf[KP][KB];
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+                const uint32_t row = 32u * b + li;
+                const uint32_t at = (row * CPR + ((2u * st + h) ^ pg_swz_k<HD>(row))) * 16u;
+#pragma unroll
+                for (int q = 0; q < KP; ++q) kf[q][b] = *reinterpret_cast<const v4u32*>(kt + q * TB + at);
+            }
+            if constexpr (F16) {
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int b = 0; b < KB; ++b)
+                        sacc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(pg_half8, kf[0][b]),
+                                                                         __builtin_bit_cast(pg_half8, qp[a][st]), sacc[b], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int a = 2; a >= 0; --a)
+#pragma unroll
+                    for (int c = 2 - a; c >= 0; --c)
+                        sacc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pg_bf8, kf[a][0]),
+                                                                          __builtin_bit_cast(pg_bf8, qp[c][st]), sacc[0], 0, 0, 0);
+            }
+        }
+        // ---- masks and running softmax of row li: keys 32 b + 8 (v / 4) + 4 h + v % 4 ----
+        const uint64_t all = KT == 64u ? ~0ull : (1ull << (KT % 64u)) - 1ull;
+        const bool full = live_now == all && (int64_t)(k0 + KT - 1u) <= first_pos;
+        if (!full) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const uint32_t key = 32u * b + 8u * (v / 4) + 4u * h + v % 4;
+                    const bool on = ((live_now >> key) & 1ull) && (int32_t)(k0 + key) <= qpos;
+                    sacc[b][v] = on ? sacc[b][v] * qf : -INFINITY;
+                }
+        } else {
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) sacc[b][v] *= qf;
+        }
+        float mx = sacc[0][0];
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sacc[b][v]);
+        {
+            const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+            mx = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
+        }
+        const float mn = fmaxf(m, mx);
+        const float mref = mn == -INFINITY ? 0.f : mn;
+        if (__ballot(mn > m)) {
+            const float f = __builtin_amdgcn_exp2f(m - mref);
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < OD; ++d)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) o[d][v] *= f;
+        }
+        m = mn;
+        v4u32 pp[NP][2 * KB];
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            float ls = 0.f;
+#pragma unroll
+            for (int v = 0; v < 16; v += 2) {
+                const float e0 = __builtin_amdgcn_exp2f(sacc[b][v] - mref + kBoost);
+                const float e1 = __builtin_amdgcn_exp2f(sacc[b][v + 1] - mref + kBoost);
+                ls += e0 + e1;
+                uint32_t w[3];
+                if constexpr (F16) pg_split2(e0, e1, &w[0], &w[1]);
+                else pg_cut2(e0, e1, &w[0], &w[1], &w[2]);
+#pragma unroll
+                for (int a = 0; a < NP; ++a) pp[a][2 * b + v / 8][(v % 8) / 2] = w[a];
+            }
+            l += ls;
+        }
+        // ---- values: keys nobody sees read as zero, and a key that only some of the rows see
+        // must not meet the others' zero weights when its values are not finite ----
+        uint64_t use = all;
+        if (!full) {
+            use = live_now;
+            uint64_t bad = 0;
+            // keys past the wave's first row
+            const int64_t ahead = first_pos + 1 - (int64_t)k0;
+            const uint64_t later = ahead >= 64 ? 0ull : ahead <= 0 ? ~0ull : ~0ull << ahead;
+            if (use & later) {
+#pragma unroll
+                for (int t4 = 0; t4 < 2 * KB; ++t4)
+#pragma unroll
+                    for (int d = 0; d < OD; ++d) {
+                        const v4u32 a = v_frag(vt, t4, d);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            // binary16: exponent of all ones; a cut float32's first part carries it
+                            const uint32_t x = (a[i / 2] >> (16 * (i % 2))) & 0xFFFFu;
+                            const uint32_t ex = F16 ? 0x7C00u : 0x7F80u;
+                            const uint64_t who = __ballot((x & ex) == ex);
+                            const uint32_t key = 16u * t4 + 8u * (i / 4) + i % 4;
+                            if (who & 0xFFFFFFFFull) bad |= 1ull << key;
+                            if (who >> 32) bad |= 1ull << (key + 4u);
+                        }
+                    }
+                bad &= use & later;
+                use &= ~bad;
+                for (uint64_t rest = bad; rest; rest &= rest - 1ull) {
+                    const uint32_t key = (uint32_t)__builtin_ctzll(rest);
+                    const uint32_t want = (key / 16u) * 8u + 4u * ((key % 16u) / 8u) + key % 4u;   // register of the weight
+                    float mine = 0.f;
+#pragma unroll
+                    for (int b = 0; b < KB; ++b)
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) {
+                            const float e = __builtin_amdgcn_exp2f(sacc[b][v] - mref + kBoost);
+                            mine = (uint32_t)(16 * b + v) == want ? e : mine;
+                        }
+                    const float w = __shfl(mine, (int)(32u * ((key / 4u) % 2u) + li), kWave);
+                    const uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)unit_now, (int)key);
+                    if ((int32_t)(k0 + key) <= qpos) {
+#pragma unroll
+                        for (int d = 0; d < OD; ++d)
+#pragma unroll
+                            for (int v = 0; v < 16; ++v) {
+                                const uint32_t dim = 32u * d + 8u * (v / 4) + 4u * h + v % 4;
+                                if (dim < hd) o[d][v] = fmaf(w, pg_value<F16>(g.v, at, dim), o[d][v]);
+                            }
+                    }
+                }
+            }
+        }
+        // ---- O^T += V^T P^T ----
+        auto values = [&](bool cut) {
+#pragma unroll
+            for (int t4 = 0; t4 < 2 * KB; ++t4) {
+                v4u32 keep = {~0u, ~0u, ~0u, ~0u};
+                if (cut) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint32_t key = 16u * t4 + 8u * (i / 4) + 4u * h + i % 4;
+                        if (!((use >> key) & 1ull)) keep[i / 2] &= i % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+                    }
+                }
+#pragma unroll
+                for (int d = 0; d < OD; ++d) {
+                    v4u32 a[KP];
+#pragma unroll
+                    for (int q = 0; q < KP; ++q) {
+                        a[q] = v_frag(vt + q * TB, t4, d);
+                        if (cut) a[q] &= keep;
+                    }
+                    if constexpr (F16) {
+#pragma unroll
+                        for (int b = 0; b < 2; ++b)
+                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(pg_half8, a[0]),
+                                                                          __builtin_bit_cast(pg_half8, pp[b][t4]), o[d], 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int q = 2; q >= 0; --q)
+#pragma unroll
+                            for (int b = 2 - q; b >= 0; --b)
+                                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pg_bf8, a[q]),
+                                                                               __builtin_bit_cast(pg_bf8, pp[b][t4]), o[d], 0, 0, 0);
+                    }
+                }
+            }
+        };
+        if (use == all) values(false);
+        else values(true);
+    }
+    {
+        const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+        l = __uint_as_float(w[0]) + __uint_as_float(w[1]);
+    }
+    if (lives > 1u) {
+        // states in lane order: piece (wave, j) of 64 lanes x 16 bytes, then m, l a lane
+        constexpr uint32_t NJ = HD / 8;
+        const uint32_t stride = it.tiles * g.KVH;
+        auto state = [&](uint32_t c) { return p.part + (uint64_t)(it.first + c * stride) * p.part_floats; };
+        if (wave_on) {
+            float* b = state(it.chunk);
+#pragma unroll
+            for (int d = 0; d < OD; ++d)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float* x = b + ((wave * NJ + 4u * d + q) * kWave + lane) * 4u;
+                    pg_put2(x, o[d][4 * q], o[d][4 * q + 1]);
+                    pg_put2(x + 2, o[d][4 * q + 2], o[d][4 * q + 3]);
+                }
+            pg_put2(b + kPgWideRows * HD + (wave * kWave + lane) * 2u, m, l);
+        }
+        if (!paged_arrive(p.count + it.first, lives, shared)) return;
+        if (!wave_on) return;
+        float mx = -INFINITY;
+        for (uint32_t c = 0; c < lives; ++c) mx = fmaxf(mx, pg_get2(state(c) + kPgWideRows * HD + (wave * kWave + lane) * 2u).x);
+        const float mf = mx == -INFINITY ? 0.f : mx;
+        l = 0.f;
+#pragma unroll
+        for (int d = 0; d < OD; ++d)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[d][v] = 0.f;
+        for (uint32_t c = 0; c < lives; ++c) {
+            const float* b = state(c);
+            const float2 ml = pg_get2(b + kPgWideRows * HD + (wave * kWave + lane) * 2u);
+            const float f = __builtin_amdgcn_exp2f(ml.x - mf);
+            l = fmaf(f, ml.y, l);
+#pragma unroll
+            for (int d = 0; d < OD; ++d) {
+                float2 x[8];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float* y = b + ((wave * NJ + 4u * d + q) * kWave + lane) * 4u;
+                    x[2 * q] = pg_get2(y);
+                    x[2 * q + 1] = pg_get2(y + 2);
+                }
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    o[d][2 * q] = fmaf(f, x[q].x, o[d][2 * q]);
+                    o[d][2 * q + 1] = fmaf(f, x[q].y, o[d][2 * q + 1]);
+                }
+            }
+        }
+    }
+    if (!wave_on || wave * 32u + li >= nrow) return;
+    const float inv = l == 0.f ? 0.f : 1.0f / l;             // a row that sees nothing: zeros
+    float* out = p.out + (uint64_t)(it.row0 + tok) * p.ldo + (uint64_t)head * hd;
+#pragma unroll
+    for (int d = 0; d < OD; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const uint32_t dim = 32u * d + 8u * q + 4u * h;
+            if (dim < hd)
+                *reinterpret_cast<float4*>(out + dim) =
+                    make_float4(o[d][4 * q] * inv, o[d][4 * q + 1] * inv, o[d][4 * q + 2] * inv, o[d][4 * q + 3] * inv);
+        }
+}
+
+// WIDE false: every sequence has at most 16 rows a KV head (single tokens), and
+// the kernel is built without the wide items' registers and LDS.
+template <int HD, bool F16, bool WIDE>
+__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnParams p) {
+    constexpr uint32_t kNarrowLds = (4u * 16u * (HD + 4u) + 128u) * 4u;
+    constexpr uint32_t kWideLds = (F16 ? 4u : 6u) * pg_wide_keys(F16) * HD * 2u;
+    __shared__ __align__(16) char smem[WIDE && kWideLds > kNarrowLds ? kWideLds : kNarrowLds];
+    __shared__ uint32_t shared;
+    PagedItem it;
+    if (!paged_item(p, blockIdx.x, &it)) return;
+    if constexpr (WIDE) {
+        if (!it.narrow) {
+            paged_wide<HD, F16>(p, it, smem, &shared);
+            return;
+        }
+    } else if (!it.narrow) {
+        return;
+    }
+    paged_narrow<HD, F16>(p, it, reinterpret_cast<float*>(smem), &shared);
 }
 
 }  // namespace qora

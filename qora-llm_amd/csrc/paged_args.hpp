@@ -75,6 +75,8 @@ inline const char* paged_kv_error(const qora_paged_kv* kv) {
         if ((n[i] - 1) > ((1ull << 58) - extent) / st[i]) return "page pool too large";
         extent += (n[i] - 1) * st[i];
     }
+    // rows are addressed in units of 16 bytes in 32 bits
+    if (extent / al >= (1ull << 32)) return "page pool larger than 64 GiB";
     if (kv->k == kv->v) return "k and v pools are the same memory";
     return nullptr;
 }

@@ -24,11 +24,50 @@ hipError_t launch_paged_append(const PagedAppendParams& in, bool f16, hipStream_
     return hipGetLastError();
 }
 
-hipError_t launch_paged_attn(const PagedAttnParams& p, bool f16, hipStream_t stream) {
+// Items the work is cut into: twice the CUs, two workgroups on each.
+static uint32_t paged_target(int cus) { return 2u * (uint32_t)std::max(1, cus); }
+
+// Items beyond the target: every tile's last chunk may be a short one.
+uint64_t paged_attn_items(uint64_t rows, uint64_t seqs, uint32_t G, uint32_t KVH, int cus) {
+    return paged_target(cus) + (uint64_t)KVH * (seqs + rows * G / kPgWideRows);
+}
+
+static bool paged_wide_rows(uint64_t max_new, uint32_t G) { return max_new * G > kPgNarrowRows; }
+
+uint64_t paged_attn_part_bytes(uint64_t rows, uint64_t seqs, uint32_t G, uint32_t KVH, uint32_t hd, int cus) {
+    return paged_attn_items(rows, seqs, G, KVH, cus) * pg_part_floats(hd <= 64 ? 64 : 128, paged_wide_rows(rows, G)) *
+           sizeof(float);
+}
+
+hipError_t launch_paged_attn(const PagedAttnParams& in, bool f16, int cus, hipStream_t stream) {
+    PagedAttnParams p = in;
     if (p.g.rows == 0 || p.g.seqs == 0) return hipSuccess;
-    const dim3 grid(p.g.rows, p.H), block(64);
-    if (f16) hipLaunchKernelGGL((paged_attn_row_kernel<true>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((paged_attn_row_kernel<false>), grid, block, 0, stream, p);
+    const uint32_t es = f16 ? 2u : 4u, HD = p.g.hd <= 64 ? 64u : 128u;
+    p.page_u = (uint32_t)(p.g.page_stride * es / 16u);
+    p.head_u = (uint32_t)(p.g.head_stride * es / 16u);
+    p.slot_u = (uint32_t)(p.g.slot_stride * es / 16u);
+    const bool wide = paged_wide_rows(p.g.max_new, p.G);
+    p.narrow_keys = pg_narrow_keys(f16);
+    p.wide_keys = pg_wide_keys(f16);
+    p.narrow_cost = 2.f;
+    p.wide_cost = 1.f;
+    p.target = (float)paged_target(cus);
+    p.least = 2.f;
+    p.part_floats = pg_part_floats(HD, wide);
+    const uint64_t items = paged_attn_items(p.g.rows, p.g.seqs, p.G, p.g.KVH, cus);
+    if (items > 0x7FFFFFFFull) return hipErrorInvalidValue;
+    const dim3 grid((uint32_t)items), block(256);
+#define QORA_PAGED(HD_, F_, W_) hipLaunchKernelGGL((paged_attn_kernel<HD_, F_, W_>), grid, block, 0, stream, p)
+#define QORA_PAGED_W(HD_, F_) \
+    do {                      \
+        if (wide) QORA_PAGED(HD_, F_, true); else QORA_PAGED(HD_, F_, false); \
+    } while (0)
+    if (HD == 128 && f16) QORA_PAGED_W(128, true);
+    else if (HD == 128) QORA_PAGED_W(128, false);
+    else if (f16) QORA_PAGED_W(64, true);
+    else QORA_PAGED_W(64, false);
+#undef QORA_PAGED_W
+#undef QORA_PAGED
     return hipGetLastError();
 }
 
