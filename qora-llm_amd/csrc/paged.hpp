@@ -320,6 +320,28 @@ __device__ __forceinline__ float pg_value(const void* pool, uint32_t unit, uint3
     else return reinterpret_cast<const float*>(b)[d];
 }
 
+// A value that the compiler takes as new here: what is derived from it below is computed
+// where it is used instead of being kept in registers over a loop.
+__device__ __forceinline__ uint32_t pg_fresh(uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+using pg_lds_p = __attribute__((address_space(3))) char*;
+template <typename T>
+__device__ __forceinline__ T pg_lds(uint32_t at) {
+    return *reinterpret_cast<__attribute__((address_space(3))) T*>(at);
+}
+
+// 16 bytes a lane from memory to LDS, lane l's to dst + 16 l (dst the same in the
+// wave), without a register between. As a statement of its own, so that LDS reads
+// of the other buffer are not held back for it: the caller waits (pg_loads_done)
+// before the barrier that hands the tile over.
+__device__ __forceinline__ void pg_load_lds(uint64_t src, uint32_t dst) {
+    const uint32_t base = __builtin_amdgcn_readfirstlane(dst);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(base), "v"(src) : "m0", "memory");
+}
+__device__ __forceinline__ void pg_loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 // ---- narrow items ----
 // Wave w takes keys NK (4 i + w) .. of the chunk, NK = 32 (float32: 16) a step.
 // Lane (g, li) = (l / 16, l % 16): the scores of row li for keys 16 c + 4 g + r
@@ -761,32 +783,28 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
         *live = __ballot(on) & (KT == 64u ? ~0ull : (1ull << (KT % 64u)) - 1ull);
         return on ? paged_row_unit(p, it.kvh, page, key % g.page_size) : it.kvh * p.head_u;
     };
-    auto row_at = [&](uint32_t unit, uint32_t key) {
-        return (uint64_t)(uint32_t)__builtin_amdgcn_ds_bpermute((int)(4u * key), (int)unit) << 4;
-    };
-    char* const kt0 = smem;                                  // binary16: [buffer]; float32: [part]
-    char* const vt0 = smem + (F16 ? 2u : 3u) * TB;
+    const uint32_t kt0 = (uint32_t)(uintptr_t)(pg_lds_p)smem;   // binary16: [buffer]; float32: [part]
+    const uint32_t vt0 = kt0 + (F16 ? 2u : 3u) * TB;
     constexpr int NL = (int)(KT * HD * ES / 16u / 256u);     // 16-byte pieces of K (and V) a thread moves
     v4u32 kreg[F16 ? 1 : NL], vreg[F16 ? 1 : NL];
     auto load_tile = [&](uint32_t unit, uint32_t buf) {
+        const uint32_t ln = pg_fresh(lane);
 #pragma unroll
         for (int j = 0; j < NL; ++j) {
-            const uint32_t n = (wave * NL + (uint32_t)j) * kWave + lane;
+            constexpr uint32_t PR = F16 ? CPR : HD / 4;       // pieces of a cache row
+            constexpr uint32_t RW = kWave / PR;               // rows of 64 pieces
+            const uint32_t row = (wave * NL + (uint32_t)j) * RW + ln / PR, c = ln % PR;
+            const uint32_t u = (uint32_t)__builtin_amdgcn_ds_bpermute((int)(4u * row), (int)unit);
             if constexpr (F16) {
-                // piece n of the tile: LDS takes a wave's pieces in lane order
-                const uint32_t row = n / CPR, c = n % CPR, ck = c ^ pg_swz_k<HD>(row), cv = c ^ pg_swz_v<HD>(row);
-                const uint64_t at = row_at(unit, row);
-                const char* ks = reinterpret_cast<const char*>(g.k) + at + (8u * ck < hd ? ck : 0u) * 16u;
-                const char* vs = reinterpret_cast<const char*>(g.v) + at + (8u * cv < hd ? cv : 0u) * 16u;
-                char* kd = kt0 + buf * TB + (wave * NL + (uint32_t)j) * 1024u;
-                char* vd = vt0 + buf * TB + (wave * NL + (uint32_t)j) * 1024u;
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(uint64_t)ks,
-                                                 (__attribute__((address_space(3))) void*)kd, 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(uint64_t)vs,
-                                                 (__attribute__((address_space(3))) void*)vd, 16, 0, 0);
+                // LDS takes a wave's pieces in lane order: the permutation is in which piece a lane loads
+                uint32_t ck = c ^ pg_swz_k<HD>(row), cv = c ^ pg_swz_v<HD>(row);
+                ck = 8u * ck < hd ? ck : 0u;
+                cv = 8u * cv < hd ? cv : 0u;
+                const uint32_t d = buf * TB + (wave * NL + (uint32_t)j) * 1024u;
+                pg_load_lds((uint64_t)g.k + ((uint64_t)(u + ck) << 4), kt0 + d);
+                pg_load_lds((uint64_t)g.v + ((uint64_t)(u + cv) << 4), vt0 + d);
             } else {
-                const uint32_t row = n / (HD / 4), c = n % (HD / 4);
-                const uint64_t at = row_at(unit, row) + (4u * c < hd ? c : 0u) * 16u;
+                const uint64_t at = (uint64_t)(u + (4u * c < hd ? c : 0u)) << 4;
                 kreg[j] = ld_global<v4u32>(reinterpret_cast<const char*>(g.k) + at);
                 vreg[j] = ld_global<v4u32>(reinterpret_cast<const char*>(g.v) + at);
             }
@@ -794,27 +812,31 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
     };
     auto store_tile = [&]() {                                // float32: three parts of four dims, 8 bytes each
         if constexpr (!F16) {
+            const uint32_t ln = pg_fresh(lane);
 #pragma unroll
             for (int j = 0; j < NL; ++j) {
-                const uint32_t n = (wave * NL + (uint32_t)j) * kWave + lane;
-                const uint32_t row = n / (HD / 4), c = n % (HD / 4);
-                const uint32_t ak = (row * CPR + ((c / 2u) ^ pg_swz_k<HD>(row))) * 16u + (c % 2u) * 8u;
-                const uint32_t av = (row * CPR + ((c / 2u) ^ pg_swz_v<HD>(row))) * 16u + (c % 2u) * 8u;
+                constexpr uint32_t PR = HD / 4, RW = kWave / PR;
+                const uint32_t row = (wave * NL + (uint32_t)j) * RW + ln / PR, c = ln % PR;
+                const uint32_t ak = kt0 + (row * CPR + ((c / 2u) ^ pg_swz_k<HD>(row))) * 16u + (c % 2u) * 8u;
+                const uint32_t av = vt0 + (row * CPR + ((c / 2u) ^ pg_swz_v<HD>(row))) * 16u + (c % 2u) * 8u;
                 uint32_t a[3], b[3];
                 pg_cut2(__uint_as_float(kreg[j][0]), __uint_as_float(kreg[j][1]), &a[0], &a[1], &a[2]);
                 pg_cut2(__uint_as_float(kreg[j][2]), __uint_as_float(kreg[j][3]), &b[0], &b[1], &b[2]);
 #pragma unroll
-                for (uint32_t q = 0; q < 3; ++q) *reinterpret_cast<uint2*>(kt0 + q * TB + ak) = make_uint2(a[q], b[q]);
+                for (uint32_t q = 0; q < 3; ++q)
+                    *reinterpret_cast<__attribute__((address_space(3))) v2u32*>(ak + q * TB) = v2u32{a[q], b[q]};
                 pg_cut2(__uint_as_float(vreg[j][0]), __uint_as_float(vreg[j][1]), &a[0], &a[1], &a[2]);
                 pg_cut2(__uint_as_float(vreg[j][2]), __uint_as_float(vreg[j][3]), &b[0], &b[1], &b[2]);
 #pragma unroll
-                for (uint32_t q = 0; q < 3; ++q) *reinterpret_cast<uint2*>(vt0 + q * TB + av) = make_uint2(a[q], b[q]);
+                for (uint32_t q = 0; q < 3; ++q)
+                    *reinterpret_cast<__attribute__((address_space(3))) v2u32*>(av + q * TB) = v2u32{a[q], b[q]};
             }
         }
     };
 
     int32_t page = page_of(kbeg), page1 = page_of(kbeg + KT);
-    v4u32 qp[NP][QS];
+    // q: its two parts; over a float32 cache the values themselves (64 registers instead of 96), cut at each use
+    v4u32 qp[2][QS];
     float qf = p.scale * 1.4426950408889634f;
     {
         float qv[QS][8], amax = 0.f;
@@ -840,11 +862,10 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
         for (int st = 0; st < QS; ++st)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                uint32_t w[3];
+                uint32_t w[2] = {__float_as_uint(qv[st][2 * i]), __float_as_uint(qv[st][2 * i + 1])};
                 if constexpr (F16) pg_split2(ldexpf(qv[st][2 * i], -e), ldexpf(qv[st][2 * i + 1], -e), &w[0], &w[1]);
-                else pg_cut2(qv[st][2 * i], qv[st][2 * i + 1], &w[0], &w[1], &w[2]);
 #pragma unroll
-                for (int a = 0; a < NP; ++a) qp[a][st][i] = w[a];
+                for (int a = 0; a < 2; ++a) qp[a][st][i] = w[a];
             }
     }
     constexpr float kBoost = F16 ? 15.f : 0.f;
@@ -859,17 +880,18 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
     uint32_t unit = unit_of(kbeg, page, &live);
     load_tile(unit, 0);
     uint32_t buf = 0;
-    // V^T piece of dim tile d, 16 keys 16 t4 .., part q: the lane's dim, keys 8 j + 4 h + r
+    // LDS places: K piece 2 st + h of key li is at kl0 ^ 32 st; the V piece of dim tile d, keys 8 j .. (with the
+    // lane's part of them) at vl0 ^ (64 d + 32 j), rows further by whole rows
+    const uint32_t kl0 = (li * CPR + (h ^ pg_swz_k<HD>(li))) * 16u;
     const uint32_t l16 = lane % 16u, vrow = 4u * h + l16 / 4u;
-    auto v_frag = [&](const char* vt, int t4, int d) {
+    const uint32_t vl0 = (vrow * CPR + ((2u * ((lane / 16u) % 2u) + (l16 % 4u) / 2u) ^ pg_swz_v<HD>(vrow))) * 16u + (l16 % 2u) * 8u;
+    auto v_frag = [&](uint32_t vl, int t4, int d) {
         v4u32 a;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const uint32_t row = 16u * t4 + 8u * j + vrow;
-            const uint32_t c = 4u * d + 2u * ((lane / 16u) % 2u) + (l16 % 4u) / 2u;
-            const char* at = vt + (row * CPR + (c ^ pg_swz_v<HD>(row))) * 16u + (l16 % 2u) * 8u;
+            const uint32_t at = (vl ^ (64u * d + 32u * j)) + (16u * t4 + 8u * j) * CPR * 16u;
             const v2u32 x = __builtin_bit_cast(v2u32, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                          (__attribute__((address_space(3))) pg_s4*)at));
+                                                          reinterpret_cast<__attribute__((address_space(3))) pg_s4*>(at)));
             a[2 * j] = x[0];
             a[2 * j + 1] = x[1];
         }
@@ -880,12 +902,13 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
             __syncthreads();                                 // the previous tile is consumed
             store_tile();
         }
-        __syncthreads();                                     // (waits for this wave's loads to LDS first)
+        if constexpr (F16) pg_loads_done();
+        __syncthreads();
         const int32_t page2 = page_of(k0 + 2u * KT);
         const uint32_t unit1 = unit_of(k0 + KT, page1, &live1);
         if (k0 + KT < kend) load_tile(unit1, buf ^ 1u);
-        const char* kt = kt0 + (F16 ? buf * TB : 0u);
-        const char* vt = vt0 + (F16 ? buf * TB : 0u);
+        const uint32_t kt = kt0 + (F16 ? buf * TB : 0u);
+        const uint32_t vt = vt0 + (F16 ? buf * TB : 0u);
         const uint64_t live_now = live;
         const uint32_t unit_now = unit;
         buf ^= 1u;
@@ -894,6 +917,7 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
         page1 = page2;
         if (!wave_on) continue;
         // ---- scores ----
+        const uint32_t kl = kt + pg_fresh(kl0);             // (a multiple of 128 bytes apart: the pieces' bits stay free)
         pg_f16 sacc[KB];
 #pragma unroll
         for (int b = 0; b < KB; ++b)
@@ -904,10 +928,9 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
             v4u32 kf[KP][KB];
 #pragma unroll
             for (int b = 0; b < KB; ++b) {
-                const uint32_t row = 32u * b + li;
-                const uint32_t at = (row * CPR + ((2u * st + h) ^ pg_swz_k<HD>(row))) * 16u;
+                const uint32_t at = (kl ^ (32u * st)) + 32u * b * CPR * 16u;
 #pragma unroll
-                for (int q = 0; q < KP; ++q) kf[q][b] = *reinterpret_cast<const v4u32*>(kt + q * TB + at);
+                for (int q = 0; q < KP; ++q) kf[q][b] = pg_lds<v4u32>(at + q * TB);
             }
             if constexpr (F16) {
 #pragma unroll
@@ -917,31 +940,39 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
                         sacc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(pg_half8, kf[0][b]),
                                                                          __builtin_bit_cast(pg_half8, qp[a][st]), sacc[b], 0, 0, 0);
             } else {
+                v4u32 qc[3];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t w[3];
+                    pg_cut2(__uint_as_float(pg_fresh(qp[0][st][i])), __uint_as_float(pg_fresh(qp[1][st][i])), &w[0], &w[1], &w[2]);
+#pragma unroll
+                    for (int a = 0; a < 3; ++a) qc[a][i] = w[a];
+                }
 #pragma unroll
                 for (int a = 2; a >= 0; --a)
 #pragma unroll
                     for (int c = 2 - a; c >= 0; --c)
                         sacc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pg_bf8, kf[a][0]),
-                                                                          __builtin_bit_cast(pg_bf8, qp[c][st]), sacc[0], 0, 0, 0);
+                                                                          __builtin_bit_cast(pg_bf8, qc[c]), sacc[0], 0, 0, 0);
             }
         }
         // ---- masks and running softmax of row li: keys 32 b + 8 (v / 4) + 4 h + v % 4 ----
         const uint64_t all = KT == 64u ? ~0ull : (1ull << (KT % 64u)) - 1ull;
         const bool full = live_now == all && (int64_t)(k0 + KT - 1u) <= first_pos;
         if (!full) {
+            const uint32_t h4 = 4u * pg_fresh(h);
+            const uint64_t there = live_now >> h4;
+            // keys up to the row's position
+            const int64_t reach = (int64_t)qpos - (int64_t)k0 - (int64_t)h4;
+            const int32_t most = (int32_t)max((int64_t)-1, min(reach, (int64_t)64));
 #pragma unroll
             for (int b = 0; b < KB; ++b)
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
-                    const uint32_t key = 32u * b + 8u * (v / 4) + 4u * h + v % 4;
-                    const bool on = ((live_now >> key) & 1ull) && (int32_t)(k0 + key) <= qpos;
-                    sacc[b][v] = on ? sacc[b][v] * qf : -INFINITY;
+                    const int key = 32 * b + 8 * (v / 4) + v % 4;
+                    const bool on = ((there >> key) & 1ull) && key <= most;
+                    sacc[b][v] = on ? sacc[b][v] : -INFINITY;
                 }
-        } else {
-#pragma unroll
-            for (int b = 0; b < KB; ++b)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) sacc[b][v] *= qf;
         }
         float mx = sacc[0][0];
 #pragma unroll
@@ -950,7 +981,7 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
             for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sacc[b][v]);
         {
             const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-            mx = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
+            mx = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])) * qf;
         }
         const float mn = fmaxf(m, mx);
         const float mref = mn == -INFINITY ? 0.f : mn;
@@ -963,25 +994,10 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
                 for (int v = 0; v < 16; ++v) o[d][v] *= f;
         }
         m = mn;
-        v4u32 pp[NP][2 * KB];
-#pragma unroll
-        for (int b = 0; b < KB; ++b) {
-            float ls = 0.f;
-#pragma unroll
-            for (int v = 0; v < 16; v += 2) {
-                const float e0 = __builtin_amdgcn_exp2f(sacc[b][v] - mref + kBoost);
-                const float e1 = __builtin_amdgcn_exp2f(sacc[b][v + 1] - mref + kBoost);
-                ls += e0 + e1;
-                uint32_t w[3];
-                if constexpr (F16) pg_split2(e0, e1, &w[0], &w[1]);
-                else pg_cut2(e0, e1, &w[0], &w[1], &w[2]);
-#pragma unroll
-                for (int a = 0; a < NP; ++a) pp[a][2 * b + v / 8][(v % 8) / 2] = w[a];
-            }
-            l += ls;
-        }
+        const float shift = kBoost - mref;                   // weight 2^(score qf - mref + boost)
         // ---- values: keys nobody sees read as zero, and a key that only some of the rows see
         // must not meet the others' zero weights when its values are not finite ----
+        const uint32_t vl = vt + pg_fresh(vl0);
         uint64_t use = all;
         if (!full) {
             use = live_now;
@@ -994,7 +1010,7 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
                 for (int t4 = 0; t4 < 2 * KB; ++t4)
 #pragma unroll
                     for (int d = 0; d < OD; ++d) {
-                        const v4u32 a = v_frag(vt, t4, d);
+                        const v4u32 a = v_frag(vl, t4, d);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             // binary16: exponent of all ones; a cut float32's first part carries it
@@ -1012,65 +1028,80 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
                     const uint32_t key = (uint32_t)__builtin_ctzll(rest);
                     const uint32_t want = (key / 16u) * 8u + 4u * ((key % 16u) / 8u) + key % 4u;   // register of the weight
                     float mine = 0.f;
+                    const float sh = __uint_as_float(pg_fresh(__float_as_uint(shift)));
 #pragma unroll
                     for (int b = 0; b < KB; ++b)
 #pragma unroll
                         for (int v = 0; v < 16; ++v) {
-                            const float e = __builtin_amdgcn_exp2f(sacc[b][v] - mref + kBoost);
+                            const float e = __builtin_amdgcn_exp2f(fmaf(sacc[b][v], qf, sh));
                             mine = (uint32_t)(16 * b + v) == want ? e : mine;
                         }
                     const float w = __shfl(mine, (int)(32u * ((key / 4u) % 2u) + li), kWave);
                     const uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)unit_now, (int)key);
                     if ((int32_t)(k0 + key) <= qpos) {
+                        const uint32_t hf = 4u * pg_fresh(h);
 #pragma unroll
                         for (int d = 0; d < OD; ++d)
 #pragma unroll
                             for (int v = 0; v < 16; ++v) {
-                                const uint32_t dim = 32u * d + 8u * (v / 4) + 4u * h + v % 4;
+                                const uint32_t dim = 32u * d + 8u * (v / 4) + hf + v % 4;
                                 if (dim < hd) o[d][v] = fmaf(w, pg_value<F16>(g.v, at, dim), o[d][v]);
+                                __builtin_amdgcn_sched_barrier(0);   // (rare: one value in a register at a time)
                             }
                     }
                 }
             }
         }
+        v4u32 pp[NP][2 * KB];
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            float ls = 0.f;
+#pragma unroll
+            for (int v = 0; v < 16; v += 2) {
+                const float e0 = __builtin_amdgcn_exp2f(fmaf(sacc[b][v], qf, shift));
+                const float e1 = __builtin_amdgcn_exp2f(fmaf(sacc[b][v + 1], qf, shift));
+                ls += e0 + e1;
+                uint32_t w[3];
+                if constexpr (F16) pg_split2(e0, e1, &w[0], &w[1]);
+                else pg_cut2(e0, e1, &w[0], &w[1], &w[2]);
+#pragma unroll
+                for (int a = 0; a < NP; ++a) pp[a][2 * b + v / 8][(v % 8) / 2] = w[a];
+            }
+            l += ls;
+        }
         // ---- O^T += V^T P^T ----
-        auto values = [&](bool cut) {
+        // (one copy of this for whole and for masked tiles: two took the registers of q)
+        const uint64_t there = use >> (4u * h);
 #pragma unroll
-            for (int t4 = 0; t4 < 2 * KB; ++t4) {
-                v4u32 keep = {~0u, ~0u, ~0u, ~0u};
-                if (cut) {
+        for (int t4 = 0; t4 < 2 * KB; ++t4) {
+            v4u32 keep = {~0u, ~0u, ~0u, ~0u};
+            if (use != all) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const uint32_t key = 16u * t4 + 8u * (i / 4) + 4u * h + i % 4;
-                        if (!((use >> key) & 1ull)) keep[i / 2] &= i % 2 ? 0x0000FFFFu : 0xFFFF0000u;
-                    }
-                }
-#pragma unroll
-                for (int d = 0; d < OD; ++d) {
-                    v4u32 a[KP];
-#pragma unroll
-                    for (int q = 0; q < KP; ++q) {
-                        a[q] = v_frag(vt + q * TB, t4, d);
-                        if (cut) a[q] &= keep;
-                    }
-                    if constexpr (F16) {
-#pragma unroll
-                        for (int b = 0; b < 2; ++b)
-                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(pg_half8, a[0]),
-                                                                          __builtin_bit_cast(pg_half8, pp[b][t4]), o[d], 0, 0, 0);
-                    } else {
-#pragma unroll
-                        for (int q = 2; q >= 0; --q)
-#pragma unroll
-                            for (int b = 2 - q; b >= 0; --b)
-                                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pg_bf8, a[q]),
-                                                                               __builtin_bit_cast(pg_bf8, pp[b][t4]), o[d], 0, 0, 0);
-                    }
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t key = 16u * t4 + 8u * (i / 4) + i % 4;
+                    if (!((there >> key) & 1ull)) keep[i / 2] &= i % 2 ? 0x0000FFFFu : 0xFFFF0000u;
                 }
             }
-        };
-        if (use == all) values(false);
-        else values(true);
+#pragma unroll
+            for (int d = 0; d < OD; ++d) {
+                v4u32 a[KP];
+#pragma unroll
+                for (int q = 0; q < KP; ++q) a[q] = v_frag(vl + q * TB, t4, d) & keep;
+                if constexpr (F16) {
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(pg_half8, a[0]),
+                                                                      __builtin_bit_cast(pg_half8, pp[b][t4]), o[d], 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int q = 2; q >= 0; --q)
+#pragma unroll
+                        for (int b = 2 - q; b >= 0; --b)
+                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pg_bf8, a[q]),
+                                                                           __builtin_bit_cast(pg_bf8, pp[b][t4]), o[d], 0, 0, 0);
+                }
+            }
+        }
     }
     {
         const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
@@ -1145,7 +1176,7 @@ template <int HD, bool F16, bool WIDE>
 __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnParams p) {
     constexpr uint32_t kNarrowLds = (4u * 16u * (HD + 4u) + 128u) * 4u;
     constexpr uint32_t kWideLds = (F16 ? 4u : 6u) * pg_wide_keys(F16) * HD * 2u;
-    __shared__ __align__(16) char smem[WIDE && kWideLds > kNarrowLds ? kWideLds : kNarrowLds];
+    __shared__ __align__(256) char smem[WIDE && kWideLds > kNarrowLds ? kWideLds : kNarrowLds];
     __shared__ uint32_t shared;
     PagedItem it;
     if (!paged_item(p, blockIdx.x, &it)) return;
