@@ -2265,8 +2265,10 @@ uint64_t pf_gemm_reserve(int fmt, uint32_t T, uint32_t K, uint32_t N, int cus) {
 
 }  // namespace
 
-extern "C" int qora_hip_gemm(qora_hip_ctx* c, uint32_t wid, const float* x, float* y, uint64_t rows, void* stream) {
-    if (!c) return QORA_HIP_E_INVALID;
+namespace {
+
+// qora_hip_gemm; with `lora` (its shape set), the adapters' two steps around the product.
+int gemm_call(qora_hip_ctx* c, uint32_t wid, const float* x, float* y, uint64_t rows, void* stream, const LoraParams* lora) {
     if (!x || !y) return fail(c, QORA_HIP_E_INVALID, "null argument");
     if (!get_weight(c, wid)) return fail(c, QORA_HIP_E_INVALID, "unknown weight id");
     DevWeight* w = &c->weights[wid];
@@ -2312,9 +2314,16 @@ extern "C" int qora_hip_gemm(qora_hip_ctx* c, uint32_t wid, const float* x, floa
         q.splits = ss.splits;
         q.kper = ss.kper;
         q.part = ss.splits > 1 ? (float*)c->ws_pf : nullptr;
+        if (lora) {
+            HIP_TRY(c, launch_lora_gemm_small(w->fmt, q, *lora, s));
+            HIP_TRY(c, launch_lora_expand(*lora, q.part, q.splits, s));
+            return QORA_HIP_OK;
+        }
         HIP_TRY(c, launch_pf_gemm_small(w->fmt, q, s));
         return QORA_HIP_OK;
     }
+    // x . A ahead of the product, which may write y over x
+    if (lora) HIP_TRY(c, launch_lora_shrink(*lora, s));
     uint8_t* base = (uint8_t*)c->ws_pf;
     uint8_t* wq = base + 2 * g.bx + g.be + g.bf + g.bs;
     float* part = g.splits > 1 ? (float*)(wq + g.bq + g.bc) : nullptr;
@@ -2341,6 +2350,7 @@ extern "C" int qora_hip_gemm(qora_hip_ctx* c, uint32_t wid, const float* x, floa
         h.kper = g.s2.kper;
         h.part = part;
         HIP_TRY(c, launch_pf_gemm2(g.s2.bm, h, s, true, q4 ? PF_W_RAW : PF_W_F16));
+        if (lora) HIP_TRY(c, launch_lora_expand(*lora, nullptr, 1, s));
         return QORA_HIP_OK;
     }
     HIP_TRY(c, launch_pf_rows(PF_ROW_SPLIT, r, T, s));
@@ -2364,7 +2374,15 @@ extern "C" int qora_hip_gemm(qora_hip_ctx* c, uint32_t wid, const float* x, floa
     h.kper = g.sh.kper;
     h.part = part;
     HIP_TRY(c, launch_pf_gemm(w->fmt, h, s));
+    if (lora) HIP_TRY(c, launch_lora_expand(*lora, nullptr, 1, s));
     return QORA_HIP_OK;
+}
+
+}  // namespace
+
+extern "C" int qora_hip_gemm(qora_hip_ctx* c, uint32_t wid, const float* x, float* y, uint64_t rows, void* stream) {
+    if (!c) return QORA_HIP_E_INVALID;
+    return gemm_call(c, wid, x, y, rows, stream, nullptr);
 }
 
 extern "C" int qora_hip_attn_prefill(qora_hip_ctx* c, const float* q, const void* kc, const void* vc, int kv_f16,
@@ -2899,7 +2917,7 @@ extern "C" int qora_hip_lora_upload(qora_hip_ctx* c, const qora_lora_adapter* ad
         };
         hipError_t e = hipSuccess;
         try {
-            if (int rc = dalloc(c, (uint64_t)max_rows * s.rp * sizeof(float), (void**)&s.u)) {
+            if (int rc = dalloc(c, (uint64_t)kLoraSlices * max_rows * s.rp * sizeof(float), (void**)&s.u)) {
                 drop();
                 return rc;
             }
@@ -2964,7 +2982,6 @@ extern "C" int qora_hip_gemm_lora(qora_hip_ctx* c, uint32_t wid, uint32_t lora_i
         if (rows == 0 || rows > s.max_rows) return fail(c, QORA_HIP_E_INVALID, "more rows than the adapters' workspace holds");
         DeviceGuard dev(c->device);
         HIP_TRY(c, dev.err);
-        const hipStream_t st = pick_stream(c, stream);
         LoraParams p{};
         p.entries = (const LoraEntry*)s.mem;
         p.count = s.count;
@@ -2976,10 +2993,7 @@ extern "C" int qora_hip_gemm_lora(qora_hip_ctx* c, uint32_t wid, uint32_t lora_i
         p.x = x;
         p.y = y;
         p.u = s.u;
-        // x . A before the product, which may write y over x
-        HIP_TRY(c, launch_lora_shrink(p, st));
-        if (int rc = qora_hip_gemm(c, wid, x, y, rows, stream)) return rc;
-        HIP_TRY(c, launch_lora_expand(p, st));
-        return QORA_HIP_OK;
+        lora_shape(&p, c->cus);
+        return gemm_call(c, wid, x, y, rows, stream, &p);
     });
 }

@@ -825,11 +825,14 @@ uint64_t pf_small_most(int fmt, uint32_t T, uint32_t n, int cus) {
     return std::max(4 * MB, 2 * cu * MB / blocks);
 }
 
+bool pf_small_ok(const PfSmallParams& p) {
+    return !(p.T == 0 || p.T > kPfSmallT || !pf_gemm_supported(p.k, p.n) || p.n % 32 != 0 || p.kper % 32 != 0 || p.kper == 0 ||
+             p.kper > (p.T > 32u ? 256u : 512u) || (uint64_t)p.splits * p.kper < p.k ||
+             (uint64_t)(p.splits - 1u) * p.kper >= p.k || p.splits > 65535u || (p.splits > 1 && !p.part));
+}
+
 hipError_t launch_pf_gemm_small(int fmt, const PfSmallParams& p, hipStream_t stream) {
-    if (p.T == 0 || p.T > kPfSmallT || !pf_gemm_supported(p.k, p.n) || p.n % 32 != 0 || p.kper % 32 != 0 || p.kper == 0 ||
-        p.kper > (p.T > 32u ? 256u : 512u) || (uint64_t)p.splits * p.kper < p.k ||
-        (uint64_t)(p.splits - 1u) * p.kper >= p.k || p.splits > 65535u || (p.splits > 1 && !p.part))
-        return hipErrorInvalidValue;
+    if (!pf_small_ok(p)) return hipErrorInvalidValue;
     const dim3 grid((p.n + 127u) / 128u, p.splits);
 #define QORA_PF_SMALL(TM_)                                                                                    \
     do {                                                                                                      \

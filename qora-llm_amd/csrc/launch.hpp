@@ -154,6 +154,7 @@ struct PfSmallShape {
 PfSmallShape pf_small_shape(uint32_t T, uint32_t k, uint32_t n, int cus);
 // the most bytes of partial sums (splits * T * n floats) for which it is the kernel to take
 uint64_t pf_small_most(int fmt, uint32_t T, uint32_t n, int cus);
+bool pf_small_ok(const PfSmallParams& p);   // a launch of it is within its bounds
 hipError_t launch_pf_gemm_small(int fmt, const PfSmallParams& p, hipStream_t stream);
 hipError_t launch_pf_rope_cache(const PrefillAttnParams& p, hipStream_t stream);
 hipError_t launch_pf_attn(const PrefillAttnParams& p, hipStream_t stream);
@@ -180,7 +181,12 @@ uint64_t paged_attn_items(uint64_t rows, uint64_t seqs, uint32_t G, uint32_t KVH
 uint64_t paged_attn_part_bytes(uint64_t rows, uint64_t seqs, uint32_t G, uint32_t KVH, uint32_t hd, int cus);
 // p.part and p.count hold that; part_floats, the strides in units and the item costs are set here.
 hipError_t launch_paged_attn(const PagedAttnParams& p, bool f16, int cus, hipStream_t stream);
+constexpr uint32_t kLoraSlices = 8;   // K slices of x . A at most
+void lora_shape(LoraParams* p, int cus);   // sets nz, kper and slots for p's k and rows
 hipError_t launch_lora_shrink(const LoraParams& p, hipStream_t stream);
-hipError_t launch_lora_expand(const LoraParams& p, hipStream_t stream);
+// launch_lora_shrink and the product kernel of launch_pf_gemm_small in one launch, without the sum over
+// q.splits slices: launch_lora_expand takes q.part and q.splits and adds them up itself (splits 1: it adds to y)
+hipError_t launch_lora_gemm_small(int fmt, const PfSmallParams& q, const LoraParams& p, hipStream_t stream);
+hipError_t launch_lora_expand(const LoraParams& p, const float* part, uint32_t splits, hipStream_t stream);
 
 }  // namespace qora

@@ -465,7 +465,9 @@ struct LoraParams {
     const int32_t* row_adapter;
     const float* x;
     float* y;
-    float* u;                  // [rows][rp]: x . A
+    float* u;                  // [nz][rows][rp]: x . A of each K slice
+    uint32_t nz, kper;         // K slices and their rows (a multiple of 32)
+    uint32_t slots;            // workgroups that share a row block's distinct adapters
 };
 
 }  // namespace qora
