@@ -2322,8 +2322,6 @@ int gemm_call(qora_hip_ctx* c, uint32_t wid, const float* x, float* y, uint64_t 
         HIP_TRY(c, launch_pf_gemm_small(w->fmt, q, s));
         return QORA_HIP_OK;
     }
-    // x . A ahead of the product, which may write y over x
-    if (lora) HIP_TRY(c, launch_lora_shrink(*lora, s));
     uint8_t* base = (uint8_t*)c->ws_pf;
     uint8_t* wq = base + 2 * g.bx + g.be + g.bf + g.bs;
     float* part = g.splits > 1 ? (float*)(wq + g.bq + g.bc) : nullptr;
@@ -2333,8 +2331,13 @@ int gemm_call(qora_hip_ctx* c, uint32_t wid, const float* x, float* y, uint64_t 
     r.xh = (uint16_t*)base;
     r.xl = (uint16_t*)(base + g.bx);
     r.xe = (int32_t*)(base + 2 * g.bx);
+    // (x . A in or ahead of the launch that prepares the product, which may write y over x)
     if (g.wide) {
-        if (q4) HIP_TRY(c, launch_pf_gemm_prep(x, T, r.xh, r.xl, r.xe, (const uint8_t*)w->w, (const uint16_t*)w->scales,
+        if (lora && !q4) HIP_TRY(c, launch_lora_shrink(*lora, s));
+        if (lora && q4)
+            HIP_TRY(c, launch_lora_gemm_prep(*lora, r.xh, r.xl, r.xe, (const uint8_t*)w->w, (const uint16_t*)w->scales,
+                                             (uint2*)wq, (uint16_t*)(wq + g.bq), s));
+        else if (q4) HIP_TRY(c, launch_pf_gemm_prep(x, T, r.xh, r.xl, r.xe, (const uint8_t*)w->w, (const uint16_t*)w->scales,
                                                K, N, (uint2*)wq, (uint16_t*)(wq + g.bq), s));
         else HIP_TRY(c, launch_pf_rows(PF_ROW_SPLIT, r, T, s));
         PfGemm2Params h{};
@@ -2349,10 +2352,11 @@ int gemm_call(qora_hip_ctx* c, uint32_t wid, const float* x, float* y, uint64_t 
         h.splits = g.s2.splits;
         h.kper = g.s2.kper;
         h.part = part;
-        HIP_TRY(c, launch_pf_gemm2(g.s2.bm, h, s, true, q4 ? PF_W_RAW : PF_W_F16));
-        if (lora) HIP_TRY(c, launch_lora_expand(*lora, nullptr, 1, s));
+        if (lora) HIP_TRY(c, launch_lora_gemm2(g.s2.bm, h, *lora, s, q4 ? PF_W_RAW : PF_W_F16));
+        else HIP_TRY(c, launch_pf_gemm2(g.s2.bm, h, s, true, q4 ? PF_W_RAW : PF_W_F16));
         return QORA_HIP_OK;
     }
+    if (lora) HIP_TRY(c, launch_lora_shrink(*lora, s));
     HIP_TRY(c, launch_pf_rows(PF_ROW_SPLIT, r, T, s));
     int8_t* wf = (int8_t*)(base + 2 * g.bx + g.be);
     if (q4)

@@ -898,22 +898,26 @@ PfGemm2Shape pf_gemm2_shape(uint32_t T, uint32_t k, uint32_t ntot, int cus) {
     return sh;
 }
 
-hipError_t launch_pf_gemm2(uint32_t bm, const PfGemm2Params& p, hipStream_t stream, bool reduce, PfW wm) {
+bool pf_gemm2_ok(uint32_t bm, const PfGemm2Params& p, PfW wm) {
     if (p.T == 0 || p.k % 32 != 0 || p.nseg < 1 || p.nseg > 3 || p.ntot % 128 != 0 || p.splits == 0 ||
         p.kper % 32 != 0 || (uint64_t)p.splits * p.kper < p.k || (p.splits > 1 && !p.part))
-        return hipErrorInvalidValue;
+        return false;
     uint32_t nb = 0;
     for (int i = 0; i < p.nseg; ++i) {
         if (p.seg[i].nb0 != nb || p.seg[i].n % 128 != 0 || !p.seg[i].wq ||
             (wm != PF_W_F16 && !p.seg[i].sc) || (wm == PF_W_PACKED && !p.seg[i].wf))
-            return hipErrorInvalidValue;
+            return false;
         nb += p.seg[i].n / 128;
     }
-    if (nb * 128u != p.ntot) return hipErrorInvalidValue;
+    if (nb * 128u != p.ntot) return false;
     if (p.swiglu && (p.nseg != 2 || p.seg[0].n != p.seg[1].n || p.splits != 1 || !p.seg[0].y || p.seg[0].accumulate))
-        return hipErrorInvalidValue;
-    const dim3 grid(nb, (p.T + bm - 1) / bm, p.splits);
-    if (bm != 32 && bm != 64) return hipErrorInvalidValue;
+        return false;
+    return bm == 32 || bm == 64;
+}
+
+hipError_t launch_pf_gemm2(uint32_t bm, const PfGemm2Params& p, hipStream_t stream, bool reduce, PfW wm) {
+    if (!pf_gemm2_ok(bm, p, wm)) return hipErrorInvalidValue;
+    const dim3 grid(p.ntot / 128u, (p.T + bm - 1) / bm, p.splits);
 #define QORA_PF_GEMM2(WM_)                                                                              \
     do {                                                                                                \
         if (bm == 64) hipLaunchKernelGGL((pf_gemm2_kernel<64, WM_>), grid, dim3(256), 0, stream, p);    \
@@ -1044,6 +1048,122 @@ hipError_t launch_pf_attn(const PrefillAttnParams& p, hipStream_t stream) {
     if (p.kv_f16) hipLaunchKernelGGL((pf_attn_vec_kernel<true>), grid, dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((pf_attn_vec_kernel<false>), grid, dim3(256), 0, stream, p);
     if (p.xh) return launch_pf_attn_split(p, stream);
+    return hipGetLastError();
+}
+
+// ---- low-rank adapters ----
+
+// K slices of the adapters' first step, of few tokens: enough workgroups for two a CU, of at
+// least 512 rows (four waves of 128), and at most eight, which the second step adds up.
+void lora_shape(LoraParams* p, int cus) {
+    const uint32_t rb = (p->rows + 15u) / 16u;
+    p->slots = rb <= 4u ? 16u : 4u;
+    p->rp32 = (p->rp + kLoraRanks - 1u) / kLoraRanks * kLoraRanks;
+    const uint32_t want = (2u * (uint32_t)std::max(1, cus) + rb * p->slots - 1u) / (rb * p->slots);
+    // (a prompt's rows: one, whose sums go out ready to multiply, in the same memory)
+    const bool few = p->rows <= kPfSmallT;
+    const uint32_t nz = few ? std::max(1u, std::min({want, (p->k + 511u) / 512u, kLoraSlices})) : 1u;
+    p->uh = few ? nullptr : reinterpret_cast<uint16_t*>(p->u);
+    p->ul = few ? nullptr : p->uh + (uint64_t)p->rows * p->rp;
+    p->ue = few ? nullptr : reinterpret_cast<int32_t*>(p->ul + (uint64_t)p->rows * p->rp);
+    p->kper = ((p->k + nz - 1u) / nz + 31u) / 32u * 32u;
+    p->nz = (p->k + p->kper - 1u) / p->kper;
+}
+
+static bool lora_ok(const LoraParams& p) {
+    return p.rows > 0 && p.k % 32 == 0 && p.n % 32 == 0 && p.kper % 32 == 0 && p.kper > 0 && p.slots > 0 && p.rp32 >= p.rp && p.rp32 % kLoraRanks == 0 &&
+           (uint64_t)p.nz * p.kper >= p.k && (uint64_t)(p.nz - 1u) * p.kper < p.k && (p.rows <= kPfSmallT) == (p.uh == nullptr);
+}
+
+__global__ __launch_bounds__(256) void lora_shrink_kernel(LoraParams p) {
+    __shared__ __align__(16) float red[kLoraShrinkLds / 4];
+    lora_shrink_block(p, blockIdx.x, blockIdx.y, blockIdx.z, red);
+}
+
+// The product's operand split and weight packing (pf_gemm_prep_kernel) and the adapters' first step in
+// one launch: both read x, and each leaves much of the chip idle by itself.
+__global__ __launch_bounds__(256, 4) void lora_gemm_prep_kernel(LoraParams p, uint32_t nshrink, uint16_t* xh, uint16_t* xl,
+                                                                int32_t* xe, const uint8_t* w, const uint16_t* scales,
+                                                                uint2* wq, uint16_t* sc) {
+    __shared__ __align__(16) float red[kLoraShrinkLds / 4];
+    if (blockIdx.x < nshrink) {
+        const uint32_t n = lora_slots(p), b = blockIdx.x / n;
+        lora_shrink_block(p, blockIdx.x % n, b % p.nz, b / p.nz, red);
+    } else {
+        pf_gemm_prep_block(blockIdx.x - nshrink, p.x, xh, xl, xe, p.rows, w, scales, p.k, p.n, wq, sc, red);
+    }
+}
+
+// The product with each row's adapter in its sums: saves the second pass over y (512 rows, 11008 columns:
+// 45 MB). As many workgroups a CU as the kernel without.
+template <int BM, int WM>
+__global__ __launch_bounds__(256, BM == 64 && WM == PF_W_F16 ? 2 : 4) void lora_gemm2_kernel(PfGemm2Params q, LoraParams p) {
+    pf_gemm2_block<BM, WM, true>(q, &p);
+}
+
+hipError_t launch_lora_gemm_prep(const LoraParams& p, uint16_t* xh, uint16_t* xl, int32_t* xe, const uint8_t* w,
+                                 const uint16_t* scales, uint2* wq, uint16_t* sc, hipStream_t stream) {
+    if (!lora_ok(p) || !pf_gemm2_supported(p.k, p.n)) return hipErrorInvalidValue;
+    const uint64_t ns = (uint64_t)lora_slots(p) * p.nz * ((p.rows + 15u) / 16u);
+    const uint64_t grid = ns + p.rows + (uint64_t)(p.n / 128u) * ((p.k / 32u + 1u) / 2u);
+    if (grid > 0x7FFFFFFFull) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(lora_gemm_prep_kernel, dim3((uint32_t)grid), dim3(256), 0, stream, p, (uint32_t)ns, xh, xl, xe, w,
+                       scales, wq, sc);
+    return hipGetLastError();
+}
+
+hipError_t launch_lora_gemm2(uint32_t bm, const PfGemm2Params& q, const LoraParams& p, hipStream_t stream, PfW wm) {
+    if (q.splits > 1) {
+        if (const hipError_t e = launch_pf_gemm2(bm, q, stream, false, wm)) return e;
+        return launch_lora_expand(p, q.part, q.splits, stream);
+    }
+    if (!lora_ok(p) || !pf_gemm2_ok(bm, q, wm) || q.nseg != 1 || q.swiglu || q.T != p.rows || q.k != p.k || q.ntot != p.n ||
+        wm == PF_W_PACKED || q.seg[0].accumulate)
+        return hipErrorInvalidValue;
+    const dim3 grid(q.ntot / 128u, (q.T + bm - 1) / bm);
+#define QORA_LORA_GEMM2(WM_)                                                                                   \
+    do {                                                                                                       \
+        if (bm == 64) hipLaunchKernelGGL((lora_gemm2_kernel<64, WM_>), grid, dim3(256), 0, stream, q, p);      \
+        else hipLaunchKernelGGL((lora_gemm2_kernel<32, WM_>), grid, dim3(256), 0, stream, q, p);               \
+    } while (0)
+    if (wm == PF_W_RAW) QORA_LORA_GEMM2(PF_W_RAW);
+    else QORA_LORA_GEMM2(PF_W_F16);
+#undef QORA_LORA_GEMM2
+    return hipGetLastError();
+}
+
+hipError_t launch_lora_shrink(const LoraParams& p, hipStream_t stream) {
+    const uint32_t rb = (p.rows + 15u) / 16u;
+    if (!lora_ok(p) || rb > 65535u) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(lora_shrink_kernel, dim3(lora_slots(p), p.nz, rb), dim3(256), 0, stream, p);
+    return hipGetLastError();
+}
+
+hipError_t launch_lora_gemm_small(int fmt, const PfSmallParams& q, const LoraParams& p, hipStream_t stream) {
+    const uint32_t rb = (p.rows + 15u) / 16u, nx = (q.n + 127u) / 128u;
+    if (!lora_ok(p) || q.T != p.rows || q.k != p.k || q.n != p.n || !pf_small_ok(q)) return hipErrorInvalidValue;
+    const uint32_t ns = lora_slots(p) * p.nz * rb;
+    const dim3 grid(ns + nx * q.splits);
+#define QORA_LORA_SMALL(TM_)                                                                                        \
+    do {                                                                                                            \
+        if (fmt == FMT_Q4) hipLaunchKernelGGL((lora_gemm_small_kernel<TM_, true>), grid, dim3(256), 0, stream, q, p, ns, nx); \
+        else hipLaunchKernelGGL((lora_gemm_small_kernel<TM_, false>), grid, dim3(256), 0, stream, q, p, ns, nx);     \
+    } while (0)
+    if (q.T <= 16u) QORA_LORA_SMALL(1);
+    else if (q.T <= 32u) QORA_LORA_SMALL(2);
+    else QORA_LORA_SMALL(4);
+#undef QORA_LORA_SMALL
+    return hipGetLastError();
+}
+
+// Up to 64 rows the waves take the adapters in turn (lora_expand_kernel<true>).
+hipError_t launch_lora_expand(const LoraParams& p, const float* part, uint32_t splits, hipStream_t stream) {
+    const uint32_t rb = (p.rows + 15u) / 16u;
+    if (!lora_ok(p) || rb > 65535u || (splits > 1u && !part)) return hipErrorInvalidValue;
+    if (p.rows <= kPfSmallT)
+        hipLaunchKernelGGL((lora_expand_kernel<true>), dim3(p.n / 32u, rb), dim3(256), 0, stream, p, part, splits);
+    else
+        hipLaunchKernelGGL((lora_expand_kernel<false>), dim3((p.n + 255u) / 256u, rb), dim3(256), 0, stream, p, part, splits);
     return hipGetLastError();
 }
 

@@ -140,6 +140,7 @@ PfGemm2Shape pf_gemm2_shape(uint32_t T, uint32_t k, uint32_t ntot, int cus);
 // p.splits, p.kper from pf_gemm2_shape (bm too); p.part holds splits * T * ntot floats when splits > 1.
 // reduce = false leaves the split partials for the consumer to sum (pf_rmsnorm_split_reg_kernel).
 // wm: PF_W_RAW for scales as launch_pf_gemm_prep packs them, PF_W_F16 for binary16 weights.
+bool pf_gemm2_ok(uint32_t bm, const PfGemm2Params& p, PfW wm);   // a launch of it is within its bounds
 hipError_t launch_pf_gemm2(uint32_t bm, const PfGemm2Params& p, hipStream_t stream, bool reduce = true,
                            PfW wm = PF_W_PACKED);
 // x [T][k] split into xh, xl, xe and a Q4 weight packed with its own scales, in one launch
@@ -182,11 +183,16 @@ uint64_t paged_attn_part_bytes(uint64_t rows, uint64_t seqs, uint32_t G, uint32_
 // p.part and p.count hold that; part_floats, the strides in units and the item costs are set here.
 hipError_t launch_paged_attn(const PagedAttnParams& p, bool f16, int cus, hipStream_t stream);
 constexpr uint32_t kLoraSlices = 8;   // K slices of x . A at most
-void lora_shape(LoraParams* p, int cus);   // sets nz, kper and slots for p's k and rows
+void lora_shape(LoraParams* p, int cus);   // sets nz, kper, slots and u's form for p's k, rows and u
 hipError_t launch_lora_shrink(const LoraParams& p, hipStream_t stream);
 // launch_lora_shrink and the product kernel of launch_pf_gemm_small in one launch, without the sum over
 // q.splits slices: launch_lora_expand takes q.part and q.splits and adds them up itself (splits 1: it adds to y)
 hipError_t launch_lora_gemm_small(int fmt, const PfSmallParams& q, const LoraParams& p, hipStream_t stream);
+// launch_pf_gemm_prep and launch_lora_shrink in one launch; launch_pf_gemm2 with the adapters' second step, in
+// its sums or with those over q.splits
+hipError_t launch_lora_gemm_prep(const LoraParams& p, uint16_t* xh, uint16_t* xl, int32_t* xe, const uint8_t* w,
+                                 const uint16_t* scales, uint2* wq, uint16_t* sc, hipStream_t stream);
+hipError_t launch_lora_gemm2(uint32_t bm, const PfGemm2Params& q, const LoraParams& p, hipStream_t stream, PfW wm);
 hipError_t launch_lora_expand(const LoraParams& p, const float* part, uint32_t splits, hipStream_t stream);
 
 }  // namespace qora

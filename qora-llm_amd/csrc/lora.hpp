@@ -63,26 +63,18 @@ __device__ __forceinline__ f32x4v lr_mma(const v4u32* x, const v4u32* w, f32x4v 
     return c;
 }
 
-// The row block's adapters: lane i % 16's row, -1 without one; and the rows that are
-// the first of their adapter, as a mask of 16.
-__device__ __forceinline__ int32_t lr_rows(const LoraParams& p, uint32_t rb, uint32_t* firsts) {
-    const uint32_t lane = threadIdx.x & (kWave - 1), i = lane % 16u, t = rb * 16u + i;
-    int32_t a = p.row_adapter[min(t, p.rows - 1u)];
-    if (t >= p.rows || a < 0 || (uint32_t)a >= p.count) a = -1;
-    bool first = a >= 0;
-#pragma unroll
-    for (uint32_t j = 0; j < 15u; ++j) {
-        const int32_t b = __builtin_amdgcn_readlane(a, (int)j);
-        if (j < i && b == a) first = false;
-    }
-    *firsts = (uint32_t)__ballot(first) & 0xFFFFu;
-    return a;
+// The adapter of row first + lane, -1 without one; lanes from `rows` on have none.
+__device__ __forceinline__ int32_t lr_mine(const LoraParams& p, uint32_t first, uint32_t rows) {
+    const uint32_t lane = threadIdx.x & (kWave - 1), t = first + lane;
+    const int32_t a = p.row_adapter[min(t, p.rows - 1u)];
+    return lane < rows && t < p.rows && a >= 0 && (uint32_t)a < p.count ? a : -1;
 }
 
-// The n-th of them.
-__device__ __forceinline__ int32_t lr_nth(int32_t mine, uint32_t firsts, uint32_t n) {
-    for (uint32_t i = 0; i < n; ++i) firsts &= firsts - 1u;
-    return __builtin_amdgcn_readlane(mine, __builtin_ctz(firsts));
+// Takes the next distinct adapter out of `rest` (lanes whose row is still to do).
+__device__ __forceinline__ int32_t lr_next(int32_t mine, uint64_t* rest) {
+    const int32_t e = __builtin_amdgcn_readlane(mine, __builtin_ctzll(*rest));
+    *rest &= ~__ballot(mine == e);
+    return e;
 }
 
 __device__ __forceinline__ LoraEntry lr_entry(const LoraParams& p, int32_t e) {
@@ -90,127 +82,297 @@ __device__ __forceinline__ LoraEntry lr_entry(const LoraParams& p, int32_t e) {
     a.at = sgpr_ptr(a.at);
     a.bt = sgpr_ptr(a.bt);
     a.rp = __builtin_amdgcn_readfirstlane(a.rp);
+    a.scale = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(a.scale)));
     return a;
 }
 
-constexpr uint32_t kLoraShrinkLds = 4u * 16u * 64u * 4u;
+constexpr uint32_t kLoraRanks = 32;                          // ranks of a workgroup of the first step
+constexpr uint32_t kLoraShrinkLds = 4u * 16u * kLoraRanks * 4u;
 
-// u[z][t][r] = sum over K slice z of x[t][k] A_e[k][r], block (slot, z, row block): the slot's
-// distinct adapters slot, slot + slots, ... Wave w takes k = 128 w .. + 127 of every 512, up to
-// 64 ranks at a time; the waves' sums are joined in LDS in wave order.
-__device__ __forceinline__ void lora_shrink_block(const LoraParams& p, uint32_t slot, uint32_t z, uint32_t rb, float* red) {
-    const uint32_t t = threadIdx.x, lane = t & (kWave - 1), g = lane / 16u, li = lane % 16u;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(t / kWave);
-    uint32_t firsts;
-    const int32_t mine = lr_rows(p, rb, &firsts);
-    const uint32_t n = (uint32_t)__popc(firsts);
-    const uint32_t kb = z * p.kper, ke = min(p.k, kb + p.kper);
-    const float* x = p.x + (uint64_t)min(rb * 16u + li, p.rows - 1u) * p.k;
-    const bool vec = pf_al(p.x, 16);
-    for (uint32_t d = slot; d < n; d += p.slots) {
-        const int32_t e = lr_nth(mine, firsts, d);
-        const LoraEntry a = lr_entry(p, e);
-        for (uint32_t c0 = 0; c0 < a.rp; c0 += 64u) {
-            f32x4v acc[4];
+// Workgroups of the first step per K slice and row block.
+__host__ __device__ __forceinline__ uint32_t lora_slots(const LoraParams& p) { return p.slots * (p.rp32 / kLoraRanks); }
+
+// A wave's part of x A^T for 16 rows and 16 NC ranks from c0 on: k = kb + 128 wave .. + 127 of every 512. x: the lane's row.
+template <bool VEC, int NC>
+__device__ __forceinline__ void lora_shrink_wave(const float* x, const LoraEntry& a, uint32_t K, uint32_t c0, uint32_t kb,
+                                                 uint32_t ke, uint32_t wave, f32x4v* acc) {
+    const uint32_t lane = threadIdx.x & (kWave - 1), g = lane / 16u, li = lane % 16u;
+    for (uint32_t k0 = kb + wave * 128u; k0 < ke; k0 += 512u) {
+        float xv[4][8];
+        v4u32 av[NC][4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) acc[c] = f32x4v{0.f, 0.f, 0.f, 0.f};
-            for (uint32_t k0 = kb + wave * 128u; k0 < ke; k0 += 512u) {
-                float xv[4][8];
-                v4u32 av[4][4];
+        for (uint32_t s = 0; s < 4; ++s) {
+            const uint32_t kc = (k0 + 32u * s < ke ? k0 + 32u * s : kb) + 8u * g;   // (k, kb and ke are multiples of 32)
+            if constexpr (VEC) {
+                const float4 u = *reinterpret_cast<const float4*>(x + kc), v = *reinterpret_cast<const float4*>(x + kc + 4);
+                xv[s][0] = u.x; xv[s][1] = u.y; xv[s][2] = u.z; xv[s][3] = u.w;
+                xv[s][4] = v.x; xv[s][5] = v.y; xv[s][6] = v.z; xv[s][7] = v.w;
+            } else {
 #pragma unroll
-                for (uint32_t s = 0; s < 4; ++s) {
-                    const uint32_t k = k0 + 32u * s + 8u * g;
-                    const bool in = k0 + 32u * s < ke;       // (k and ke are multiples of 32)
-                    const uint32_t kc = in ? k : kb + 8u * g;
-                    if (vec) {
-                        const float4 u = *reinterpret_cast<const float4*>(x + kc), v = *reinterpret_cast<const float4*>(x + kc + 4);
-                        xv[s][0] = u.x; xv[s][1] = u.y; xv[s][2] = u.z; xv[s][3] = u.w;
-                        xv[s][4] = v.x; xv[s][5] = v.y; xv[s][6] = v.z; xv[s][7] = v.w;
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) xv[s][i] = x[kc + i];
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) xv[s][i] = in ? xv[s][i] : 0.f;
-#pragma unroll
-                    for (uint32_t c = 0; c < 4; ++c)
-                        if (c0 + 16u * c < a.rp)
-                            av[c][s] = ld_global<v4u32>(a.at + (uint64_t)(c0 + 16u * c + li) * p.k + kc);
-                }
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    v4u32 xp[3];
-                    lr_cut(xv[s], xp);
-#pragma unroll
-                    for (uint32_t c = 0; c < 4; ++c)
-                        if (c0 + 16u * c < a.rp) {
-                            v4u32 wp[2];
-                            lr_cut16(av[c][s], wp);
-                            acc[c] = lr_mma(xp, wp, acc[c]);
-                        }
-                }
+                for (int i = 0; i < 8; ++i) xv[s][i] = x[kc + i];
             }
-            __syncthreads();                                 // (red is read from the round before)
 #pragma unroll
-            for (uint32_t c = 0; c < 4; ++c)
-                *reinterpret_cast<f32x4v*>(red + wave * 1024u + (16u * c + li) * 16u + 4u * g) = acc[c];
-            __syncthreads();
+            for (uint32_t c = 0; c < NC; ++c)
+                av[c][s] = ld_global<v4u32>(a.at + (uint64_t)min(c0 + 16u * c + li, a.rp - 1u) * K + kc);
+        }
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                // (column-major: a lane's four rows are one 16-byte store)
-                const uint32_t row = t % 16u, c = t / 16u + 16u * i, at = c * 16u + row;
-                const int32_t whose = __shfl(mine, (int)row, kWave);
-                if (whose == e && c0 + c < a.rp)
-                    p.u[((uint64_t)z * p.rows + rb * 16u + row) * p.rp + c0 + c] =
-                        ((red[at] + red[1024u + at]) + red[2048u + at]) + red[3072u + at];
+        for (uint32_t s = 0; s < 4; ++s) {
+            const bool in = k0 + 32u * s < ke;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) xv[s][i] = in ? xv[s][i] : 0.f;
+            v4u32 xp[3];
+            lr_cut(xv[s], xp);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                v4u32 wp[2];
+                lr_cut16(av[c][s], wp);
+                acc[c] = lr_mma(xp, wp, acc[c]);
             }
         }
     }
 }
 
-__global__ __launch_bounds__(256) void lora_shrink_kernel(LoraParams p) {
-    __shared__ __align__(16) float red[kLoraShrinkLds / 4];
-    lora_shrink_block(p, blockIdx.x, blockIdx.y, blockIdx.z, red);
+// u[z][t][r] = sum over K slice z of x[t][k] A_e[k][r], block (slot, z, row block): the slot's
+// distinct adapters slot / chunks, + slots, ... of 32 ranks (chunk slot % chunks); the waves' sums are joined in
+// LDS in wave order. With one slice and p.uh set they go out as two binary16 parts on a
+// power-of-two scale of the row's 32 (uh, ul, ue): the second step of a prompt reads them once per column block,
+// and then multiplies what it loads. VEC: x starts on 16 bytes.
+template <bool VEC>
+__device__ __forceinline__ void lora_shrink_rows(const LoraParams& p, uint32_t slot, uint32_t z, uint32_t rb, float* red) {
+    const uint32_t t = threadIdx.x, lane = t & (kWave - 1), g = lane / 16u, li = lane % 16u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(t / kWave);
+    const int32_t mine = lr_mine(p, rb * 16u, 16u);
+    uint64_t rest = __ballot(mine >= 0);
+    const uint32_t kb = z * p.kper, ke = min(p.k, kb + p.kper);
+    const float* x = p.x + (uint64_t)min(rb * 16u + li, p.rows - 1u) * p.k;
+    const uint32_t chunks = p.rp32 / kLoraRanks, c0 = (slot % chunks) * kLoraRanks;
+    slot /= chunks;
+    {
+        for (uint32_t d = 0; rest; ++d) {
+            const int32_t e = lr_next(mine, &rest);
+            if (d % p.slots != slot) continue;
+            const LoraEntry a = lr_entry(p, e);
+            if (c0 >= a.rp) continue;
+            f32x4v acc[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) acc[c] = f32x4v{0.f, 0.f, 0.f, 0.f};
+            if (a.rp - c0 <= 16u) lora_shrink_wave<VEC, 1>(x, a, p.k, c0, kb, ke, wave, acc);
+            else lora_shrink_wave<VEC, 2>(x, a, p.k, c0, kb, ke, wave, acc);
+            __syncthreads();                                 // (red is read from the round before)
+#pragma unroll
+            for (uint32_t c = 0; c < 2; ++c)
+                *reinterpret_cast<f32x4v*>(red + wave * 512u + (16u * c + li) * 16u + 4u * g) = acc[c];
+            __syncthreads();
+            // (column-major: a lane's four rows are one 16-byte store)
+            const uint32_t row = t % 16u;
+            const bool keep = __shfl(mine, (int)row, kWave) == e;
+            float v[2], amax = 0.f;
+#pragma unroll
+            for (uint32_t i = 0; i < 2; ++i) {
+                const uint32_t at = (t / 16u + 16u * i) * 16u + row;
+                v[i] = ((red[at] + red[512u + at]) + red[1024u + at]) + red[1536u + at];
+                if (c0 + t / 16u + 16u * i < a.rp) amax = fmaxf(amax, fabsf(v[i]));
+            }
+            const uint64_t r = rb * 16u + row;
+            if (!p.uh) {
+#pragma unroll
+                for (uint32_t i = 0; i < 2; ++i) {
+                    const uint32_t c = c0 + t / 16u + 16u * i;
+                    if (keep && c < a.rp) p.u[((uint64_t)z * p.rows + r) * p.rp + c] = v[i];
+                }
+                continue;
+            }
+            __syncthreads();
+            red[t] = amax;
+            __syncthreads();
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) amax = fmaxf(amax, red[16u * i + row]);
+            const int ex = pf_row_exponent(amax);
+            if (keep && t < 16u) p.ue[r * chunks + c0 / kLoraRanks] = ex;
+#pragma unroll
+            for (uint32_t i = 0; i < 2; ++i) {
+                const uint32_t c = c0 + t / 16u + 16u * i;
+                if (keep && c < a.rp)
+                    pf_split(v[i], ex, reinterpret_cast<_Float16*>(p.uh) + r * p.rp + c,
+                             reinterpret_cast<_Float16*>(p.ul) + r * p.rp + c);
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void lora_shrink_block(const LoraParams& p, uint32_t slot, uint32_t z, uint32_t rb, float* red) {
+    if (pf_al(p.x, 16)) lora_shrink_rows<true>(p, slot, z, rb, red);
+    else lora_shrink_rows<false>(p, slot, z, rb, red);
 }
 
 // The few-token GEMM and the adapters' first step in one launch: the first
-// p.slots * p.nz * row blocks workgroups are the latter's.
+// lora_slots(p) * p.nz * row blocks workgroups are the latter's.
 template <int TM, bool Q4>
 __global__ __launch_bounds__(256) void lora_gemm_small_kernel(PfSmallParams q, LoraParams p, uint32_t nshrink, uint32_t nx) {
     __shared__ __align__(16) char smem[PfSmallLds<TM, Q4>::bytes > kLoraShrinkLds ? PfSmallLds<TM, Q4>::bytes : kLoraShrinkLds];
     if (blockIdx.x < nshrink) {
-        const uint32_t b = blockIdx.x / p.slots;
-        lora_shrink_block(p, blockIdx.x % p.slots, b % p.nz, b / p.nz, reinterpret_cast<float*>(smem));
+        const uint32_t n = lora_slots(p), b = blockIdx.x / n;
+        lora_shrink_block(p, blockIdx.x % n, b % p.nz, b / p.nz, reinterpret_cast<float*>(smem));
     } else {
         const uint32_t b = blockIdx.x - nshrink;
         pf_gemm_small_block<TM, Q4>(q, b % nx, b / nx, smem);
     }
 }
 
-// y[t][j] += s_e sum_r u[t][r] B_e[r][j], block (columns, row block).
+// s_e u B_e of 16 TM rows first .. and CT 16-column tiles from u's two binary16 parts (B as it is, two products
+// of v_mfma_f32_16x16x32_f16): add() takes a value of the product for row 16 i + 4 (lane / 16) + r and tile c.
+// mine: lr_mine of the rows; cols as below.
+template <int TM, int CT>
+struct LoraTile {
+    f32x4v sum[TM][CT];
+    bool has[TM][4];
+
+    __device__ __forceinline__ float add(float v, int i, int r, int c) const { return has[i][r] ? v + sum[i][c][r] : v; }
+
+    __device__ __forceinline__ void get(const LoraParams& p, uint32_t first, int32_t mine, const uint32_t* cols) {
+        const uint32_t lane = threadIdx.x & (kWave - 1), g = lane / 16u, li = lane % 16u;
+        int32_t own[TM];
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            own[i] = __shfl(mine, (int)(16u * i + li), kWave);
+#pragma unroll
+            for (int c = 0; c < CT; ++c) sum[i][c] = f32x4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int r = 0; r < 4; ++r) has[i][r] = __shfl(mine, (int)(16u * i + 4u * g + r), kWave) >= 0;
+        }
+        const uint32_t nch = p.rp32 / kLoraRanks;
+        uint64_t rest = __ballot(mine >= 0);
+        while (rest) {
+            const int32_t e = lr_next(mine, &rest);
+            const LoraEntry a = lr_entry(p, e);
+            for (uint32_t c0 = 0; c0 < a.rp; c0 += 2u * kLoraRanks) {
+                v4u32 bv[2][CT], uh[2][TM], ul[2][TM];
+                int ex[2][TM][4];
+#pragma unroll
+                for (uint32_t s = 0; s < 2; ++s) {
+                    const uint32_t rc = min(c0 + kLoraRanks * s + 8u * g, a.rp - 8u);
+#pragma unroll
+                    for (int c = 0; c < CT; ++c) bv[s][c] = ld_global<v4u32>(a.bt + (uint64_t)min(cols[c], p.n - 1u) * a.rp + rc);
+#pragma unroll
+                    for (int i = 0; i < TM; ++i) {
+                        const uint64_t at = (uint64_t)min(first + 16u * i + li, p.rows - 1u) * p.rp + rc;
+                        uh[s][i] = ld_global<v4u32>(p.uh + at);
+                        ul[s][i] = ld_global<v4u32>(p.ul + at);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            ex[s][i][r] = p.ue[(uint64_t)min(first + 16u * i + 4u * g + r, p.rows - 1u) * nch +
+                                               min(c0 / kLoraRanks + s, nch - 1u)];
+                    }
+                }
+#pragma unroll
+                for (uint32_t s = 0; s < 2; ++s) {
+                    const bool in = c0 + kLoraRanks * s + 8u * g < a.rp;
+                    if (c0 + kLoraRanks * s >= a.rp) break;
+#pragma unroll
+                    for (int i = 0; i < TM; ++i) {
+                        // (rows of other adapters, and ranks past rp, may hold anything)
+                        const uint32_t keep = own[i] == e && in ? ~0u : 0u;
+                        bool mine_r[4];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            uh[s][i][x] &= keep;
+                            ul[s][i][x] &= keep;
+                            mine_r[x] = __shfl(mine, (int)(16u * i + 4u * g + x), kWave) == e;
+                        }
+#pragma unroll
+                        for (int c = 0; c < CT; ++c) {
+                            const half8v b = __builtin_bit_cast(half8v, bv[s][c]);
+                            f32x4v acc = f32x4v{0.f, 0.f, 0.f, 0.f};
+                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8v, ul[s][i]), b, acc, 0, 0, 0);
+                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8v, uh[s][i]), b, acc, 0, 0, 0);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                sum[i][c][r] = mine_r[r] ? sum[i][c][r] + a.scale * ldexpf(acc[r], ex[s][i][r]) : sum[i][c][r];
+                        }
+                    }
+                }
+            }
+        }
+    }
+};
+
+// u B_e (without the scale) of 16 rows first .., whose adapters `mine` holds (lr_mine), from the K slices' sums; cols[c]:
+// the column whose B this lane holds in tile c (past n: any that is not used). The rows' distinct adapters from
+// number d0 on, every step-th.
+template <int CT>
+__device__ __forceinline__ void lora_few_tile(const LoraParams& p, uint32_t first, int32_t mine, const uint32_t* cols,
+                                              f32x4v* acc, uint32_t d0, uint32_t step) {
+    const uint32_t lane = threadIdx.x & (kWave - 1), g = lane / 16u, li = lane % 16u;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) acc[c] = f32x4v{0.f, 0.f, 0.f, 0.f};
+    const int32_t own = __shfl(mine, (int)li, kWave);
+    uint64_t rest = __ballot(mine >= 0);
+    for (uint32_t d = 0; rest; ++d) {
+        const int32_t e = lr_next(mine, &rest);
+        if (d % step != d0) continue;
+        const LoraEntry a = lr_entry(p, e);
+        for (uint32_t r0 = 0; r0 < a.rp; r0 += 32u) {
+            const bool in = r0 + 8u * g < a.rp;
+            const uint32_t rc = in ? r0 + 8u * g : 0u;
+            v4u32 bv[CT];
+#pragma unroll
+            for (int c = 0; c < CT; ++c) bv[c] = ld_global<v4u32>(a.bt + (uint64_t)min(cols[c], p.n - 1u) * a.rp + rc);
+            float uv[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            for (uint32_t z0 = 0; z0 < p.nz; z0 += 4u) {     // four slices in flight
+                float4 u[4], v[4];
+#pragma unroll
+                for (uint32_t z = 0; z < 4; ++z) {
+                    const uint64_t row = (uint64_t)min(z0 + z, p.nz - 1u) * p.rows + min(first + li, p.rows - 1u);
+                    u[z] = *reinterpret_cast<const float4*>(p.u + row * p.rp + rc);
+                    v[z] = *reinterpret_cast<const float4*>(p.u + row * p.rp + rc + 4);
+                }
+#pragma unroll
+                for (uint32_t z = 0; z < 4; ++z) {
+                    if (z0 + z >= p.nz) continue;
+                    uv[0] += u[z].x; uv[1] += u[z].y; uv[2] += u[z].z; uv[3] += u[z].w;
+                    uv[4] += v[z].x; uv[5] += v[z].y; uv[6] += v[z].z; uv[7] += v[z].w;
+                }
+            }
+            // (rows of other adapters, and ranks past rp, may hold anything)
+#pragma unroll
+            for (int x = 0; x < 8; ++x) uv[x] = own == e && in ? uv[x] : 0.f;
+            v4u32 up[3];
+            lr_cut(uv, up);
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                v4u32 w = bv[c], wp[2];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) w[x] = in ? w[x] : 0u;
+                lr_cut16(w, wp);
+                acc[c] = lr_mma(up, wp, acc[c]);
+            }
+        }
+    }
+}
+
+// y[t][j] = product + s_e sum_r u[t][r] B_e[r][j], block (columns, row block); the product is y or, with
+// splits > 1, the sum of its K slices in part, in the order of the kernels that sum them without adapters.
 // FEW: 32 columns, the four waves taking the distinct adapters in turn and joining their
 // sums (single tokens: up to 16 adapters a block, so few that the columns have to fill the
-// chip); y is the sum of q.splits K slices of the product when q.splits > 1, in
-// pf_sum_splits_kernel's order. Else 64 columns a wave.
+// chip). Else 64 columns a wave.
 template <bool FEW>
 __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p, const float* part, uint32_t splits) {
-    constexpr uint32_t CT = FEW ? 2 : 4;                     // 16-column tiles of a wave
+    constexpr int CT = FEW ? 2 : 4;                          // 16-column tiles of a wave
     __shared__ __align__(16) float red[FEW ? 4 * 16 * 32 : 4];
     const uint32_t t = threadIdx.x, lane = t & (kWave - 1), g = lane / 16u, li = lane % 16u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(t / kWave);
     const uint32_t rb = blockIdx.y, n0 = FEW ? blockIdx.x * 32u : blockIdx.x * 256u + wave * 64u;
-    uint32_t firsts;
-    const int32_t mine = lr_rows(p, rb, &firsts);
-    const uint32_t n = (uint32_t)__popc(firsts);
-    if (!FEW && (n == 0 || n0 >= p.n)) return;
-    const float scale = mine >= 0 ? p.entries[mine].scale : 0.f;
-    // FEW: the product's values of this thread's two outputs, on their way while the adapters are
-    const uint32_t row2 = t / 16u, col2 = n0 + 2u * (t % 16u);
-    const uint64_t at2 = (uint64_t)min(rb * 16u + row2, p.rows - 1u) * p.n + min(col2, p.n - 2u);
-    float y0 = 0.f, y1 = 0.f;
+    const uint64_t total = (uint64_t)p.rows * p.n;
+    uint32_t cols[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) cols[c] = n0 + 16u * c + li;
+    const int32_t mine = lr_mine(p, rb * 16u, 16u);
     if constexpr (FEW) {
+        // the product's values of this thread's two outputs, on their way while the adapters are
+        const uint32_t row2 = t / 16u, col2 = n0 + 2u * (t % 16u);
+        const uint64_t at2 = (uint64_t)min(rb * 16u + row2, p.rows - 1u) * p.n + min(col2, p.n - 2u);
+        float y0 = 0.f, y1 = 0.f;
         if (splits > 1u) {
-            const uint64_t total = (uint64_t)p.rows * p.n;
             for (uint32_t z = 0; z < splits; z += 4u) {
                 float2 q[4];
 #pragma unroll
@@ -226,72 +388,42 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p, const fl
             y0 = p.y[at2];
             y1 = p.y[at2 + 1];
         }
-    }
-    f32x4v acc[CT];
+        f32x4v acc[CT];
+        lora_few_tile<CT>(p, rb * 16u, mine, cols, acc, wave, 4u);
 #pragma unroll
-    for (uint32_t c = 0; c < CT; ++c) acc[c] = f32x4v{0.f, 0.f, 0.f, 0.f};
-    for (uint32_t d = FEW ? wave : 0u; d < n; d += FEW ? 4u : 1u) {
-        const int32_t e = lr_nth(mine, firsts, d);
-        const LoraEntry a = lr_entry(p, e);
-        const bool own = mine == e;
-        for (uint32_t r0 = 0; r0 < a.rp; r0 += 32u) {
-            const bool in = r0 + 8u * g < a.rp;
-            const uint32_t rc = in ? r0 + 8u * g : 0u;
-            v4u32 bv[CT];
-#pragma unroll
-            for (uint32_t c = 0; c < CT; ++c)
-                bv[c] = ld_global<v4u32>(a.bt + (uint64_t)min(n0 + 16u * c + li, p.n - 1u) * a.rp + rc);
-            float uv[8];
-            const float* ur = p.u + (uint64_t)min(rb * 16u + li, p.rows - 1u) * p.rp + rc;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) uv[i] = 0.f;
-            for (uint32_t z = 0; z < p.nz; ++z) {
-                const float4 u = *reinterpret_cast<const float4*>(ur + (uint64_t)z * p.rows * p.rp);
-                const float4 v = *reinterpret_cast<const float4*>(ur + (uint64_t)z * p.rows * p.rp + 4);
-                uv[0] += u.x; uv[1] += u.y; uv[2] += u.z; uv[3] += u.w;
-                uv[4] += v.x; uv[5] += v.y; uv[6] += v.z; uv[7] += v.w;
-            }
-            // (rows of other adapters, and ranks past rp, may hold anything)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) uv[i] = own && in ? uv[i] : 0.f;
-            v4u32 up[3];
-            lr_cut(uv, up);
-#pragma unroll
-            for (uint32_t c = 0; c < CT; ++c) {
-                v4u32 wp[2], w = bv[c];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = in ? w[i] : 0u;
-                lr_cut16(w, wp);
-                acc[c] = lr_mma(up, wp, acc[c]);
-            }
-        }
-    }
-    if constexpr (FEW) {
-#pragma unroll
-        for (uint32_t c = 0; c < CT; ++c)
+        for (int c = 0; c < CT; ++c)
             *reinterpret_cast<f32x4v*>(red + wave * 512u + (16u * c + li) * 16u + 4u * g) = acc[c];
         __syncthreads();
         if (rb * 16u + row2 >= p.rows || col2 >= p.n) return;
         const uint32_t at = 2u * (t % 16u) * 16u + row2, bt = at + 16u;   // (column-major)
-        const float s = __shfl(scale, (int)row2, kWave);
-        const bool has = __shfl(mine, (int)row2, kWave) >= 0;
-        if (has) {
+        const int32_t e = p.row_adapter[rb * 16u + row2];
+        if (e >= 0 && (uint32_t)e < p.count) {
             // (a row has one adapter: one wave's sum, the others are zero)
-            y0 += s * ((red[at] + red[512u + at]) + (red[1024u + at] + red[1536u + at]));
-            y1 += s * ((red[bt] + red[512u + bt]) + (red[1024u + bt] + red[1536u + bt]));
+            const float s = p.entries[e].scale;
+            y0 = fmaf(s, (red[at] + red[512u + at]) + (red[1024u + at] + red[1536u + at]), y0);
+            y1 = fmaf(s, (red[bt] + red[512u + bt]) + (red[1024u + bt] + red[1536u + bt]), y1);
         }
         p.y[at2] = y0;
         p.y[at2 + 1] = y1;
     } else {
+        if (n0 >= p.n) return;
+        LoraTile<1, CT> low;
+        low.get(p, rb * 16u, mine, cols);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const uint32_t row = rb * 16u + 4u * g + r;
-            const float s = __shfl(scale, (int)(4u * g + r), kWave);
-            const bool has = __shfl(mine, (int)(4u * g + r), kWave) >= 0;
 #pragma unroll
-            for (uint32_t c = 0; c < CT; ++c) {
-                const uint32_t col = n0 + 16u * c + li;
-                if (row < p.rows && has && col < p.n) p.y[(uint64_t)row * p.n + col] += s * acc[c][r];
+            for (int c = 0; c < CT; ++c) {
+                if (row >= p.rows || cols[c] >= p.n || (splits <= 1u && !low.has[0][r])) continue;
+                const uint64_t at = (uint64_t)row * p.n + cols[c];
+                float v;
+                if (splits > 1u) {
+                    v = part[at];
+                    for (uint32_t z = 1; z < splits; ++z) v += part[(uint64_t)z * total + at];
+                } else {
+                    v = p.y[at];
+                }
+                p.y[at] = low.add(v, 0, r, c);
             }
         }
     }

@@ -461,13 +461,16 @@ struct LoraEntry {
 struct LoraParams {
     const LoraEntry* entries;
     uint32_t count, k, n, rows;
-    uint32_t rp;               // the largest rp
+    uint32_t rp, rp32;         // the largest rp, and that rounded up to 32
     const int32_t* row_adapter;
     const float* x;
     float* y;
-    float* u;                  // [nz][rows][rp]: x . A of each K slice
+    float* u;                  // [nz][rows][rp]: x . A of each K slice; or, nz = 1, in two binary16 parts
+    uint16_t* uh;              // [rows][rp] with the exponents ue [rows][rp32 / 32] (null: u)
+    uint16_t* ul;
+    int32_t* ue;
     uint32_t nz, kper;         // K slices and their rows (a multiple of 32)
-    uint32_t slots;            // workgroups that share a row block's distinct adapters
+    uint32_t slots;            // workgroups (times rp32 / 32) that share a row block's distinct adapters
 };
 
 }  // namespace qora

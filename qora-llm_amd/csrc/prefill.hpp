@@ -35,6 +35,7 @@
 
 #include "common.hpp"
 #include "params.hpp"
+#include "lora.hpp"
 #include "prefill_small.hpp"
 
 namespace qora {
@@ -582,15 +583,14 @@ __global__ __launch_bounds__(256) void pf_pack_q4_kernel(const uint8_t* w, const
 // bound by their memory traffic (512 x 2048 -> 11008: 4.2 + 8.4 MB of x and
 // 28.5 MB of weights); as separate launches behind two that found the
 // groups' largest scales they took half as long as the GEMM.
-__global__ __launch_bounds__(256) void pf_gemm_prep_kernel(const float* x, uint16_t* xh_, uint16_t* xl_, int32_t* xe, uint32_t T,
-                                                           const uint8_t* w, const uint16_t* scales, uint32_t k,
-                                                           uint32_t n, uint2* wq, uint16_t* sc) {
-    __shared__ float red[4];
+__device__ __forceinline__ void pf_gemm_prep_block(uint32_t block, const float* x, uint16_t* xh_, uint16_t* xl_,
+                                                   int32_t* xe, uint32_t T, const uint8_t* w, const uint16_t* scales,
+                                                   uint32_t k, uint32_t n, uint2* wq, uint16_t* sc, float* red) {
     const uint32_t t = threadIdx.x;
-    if (blockIdx.x < T) {
-        const float* xr = x + (uint64_t)blockIdx.x * k;
-        _Float16* xh = reinterpret_cast<_Float16*>(xh_) + (uint64_t)blockIdx.x * k;
-        _Float16* xl = reinterpret_cast<_Float16*>(xl_) + (uint64_t)blockIdx.x * k;
+    if (block < T) {
+        const float* xr = x + (uint64_t)block * k;
+        _Float16* xh = reinterpret_cast<_Float16*>(xh_) + (uint64_t)block * k;
+        _Float16* xl = reinterpret_cast<_Float16*>(xl_) + (uint64_t)block * k;
         const bool vec = pf_al(x, 16);              // k % 32 == 0, the workspace rows are aligned
         float v[8][4];
         float amax = 0.f;
@@ -619,11 +619,11 @@ __global__ __launch_bounds__(256) void pf_gemm_prep_kernel(const float* x, uint1
 #pragma unroll
             for (int i = 0; i < 8; ++i) pf_split4<true>(v[i], e, xh, xl, j0 + 4u * (t + 256u * (uint32_t)i), k);
         }
-        if (t == 0) xe[blockIdx.x] = e;
+        if (t == 0) xe[block] = e;
         return;
     }
     const uint32_t KS = k / 32u, kb2 = (KS + 1u) / 2u;
-    const uint32_t b = blockIdx.x - T, nb = b / kb2, ks0 = (b % kb2) * 2u;
+    const uint32_t b = block - T, nb = b / kb2, ks0 = (b % kb2) * 2u;
     const uint32_t bc = t % 64u, rg = t / 64u;
     const uint32_t c0 = nb * 128u + (bc / 16u) * 32u + bc % 16u, c1 = c0 + 16u;
     const uint32_t sh = (c0 & 1u) * 4u;             // column c is the low nibble of byte c / 2 when c is even
@@ -650,6 +650,13 @@ __global__ __launch_bounds__(256) void pf_gemm_prep_kernel(const float* x, uint1
             sc[(((uint64_t)nb * KS + ks) * 4u + g) * 32u + r] = scales[(uint64_t)(ks * 32u + r) * (n / 32u) + nb * 4u + g];
         }
     }
+}
+
+__global__ __launch_bounds__(256) void pf_gemm_prep_kernel(const float* x, uint16_t* xh_, uint16_t* xl_, int32_t* xe, uint32_t T,
+                                                           const uint8_t* w, const uint16_t* scales, uint32_t k,
+                                                           uint32_t n, uint2* wq, uint16_t* sc) {
+    __shared__ float red[4];
+    pf_gemm_prep_block(blockIdx.x, x, xh_, xl_, xe, T, w, scales, k, n, wq, sc, red);
 }
 
 // part[z][total] summed over z in order into y (total a multiple of 4, part
@@ -701,8 +708,11 @@ __global__ __launch_bounds__(256) void pf_sum_splits_kernel(const float* part, u
 // cache) and 1.97e-5 (f16), against 1.12e-6 and 1.81e-5 through pf_gemm_kernel and 1.35e-6
 // and 2.72e-5 with whole chains; 300 tokens 11008 -> 2048 1.7e-7 against 4.0e-7.
 // The adds cost 0 to 3% (prompts of 40 to 512 tokens through eight layers).
-template <int BM, int WM>
-__global__ __launch_bounds__(256, 2) void pf_gemm2_kernel(PfGemm2Params p) {
+// LORA (one segment, K unsplit): the sums start from each row's low-rank adapter's part
+// on the product's scale 2^-(e_t + f_g), an exact step (in the epilogue its registers would
+// halve the workgroups a CU holds: 113 against 62 us for the kernel).
+template <int BM, int WM, bool LORA>
+__device__ __forceinline__ void pf_gemm2_block(const PfGemm2Params& p, const LoraParams* lora) {
     constexpr bool RAW = WM == PF_W_RAW, F16 = WM == PF_W_F16;
     constexpr int BN = 128, KC = 32;
     constexpr uint32_t kFold = 256;
@@ -850,6 +860,28 @@ __global__ __launch_bounds__(256, 2) void pf_gemm2_kernel(PfGemm2Params p) {
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = f32x4v{0.f, 0.f, 0.f, 0.f};
+    if constexpr (LORA) {
+        uint32_t cols[TN];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) cols[j] = lnb * (uint32_t)BN + (uint32_t)wave * 32u + lcol(j);
+        // (32 rows at a time: more would not leave the registers of four workgroups a CU)
+#pragma unroll
+        for (int i0 = 0; i0 < TM; i0 += 2) {
+            const uint32_t first = m0 + (uint32_t)i0 * 16u;
+            LoraTile<2, TN> low;
+            low.get(*lora, first, lr_mine(*lora, first, 32u), cols);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int e = -(p.xe[min(first + (uint32_t)i * 16u + kq * 4u + (uint32_t)r, p.T - 1u)] + fw);
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+                        acc[i0 + i][j][r] = low.has[i][r] ? ldexpf(low.sum[i][j][r], e) : 0.f;
+                }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
     // F16: the sums of whole runs of kFold rows, which leave acc there, so that no fp32
     // chain is longer
     f32x4v tot[F16 ? TM : 1][TN];
@@ -1004,6 +1036,11 @@ __global__ __launch_bounds__(256, 2) void pf_gemm2_kernel(PfGemm2Params p) {
             }
         }
     }
+}
+
+template <int BM, int WM>
+__global__ __launch_bounds__(256, 2) void pf_gemm2_kernel(PfGemm2Params p) {
+    pf_gemm2_block<BM, WM, false>(p, nullptr);
 }
 
 // Split-K partials of pf_gemm2_kernel summed in split order, stored or added

@@ -1,6 +1,5 @@
 // Kernel instantiations and launch helpers of the many-request calls (gfx950).
 #include "launch.hpp"
-#include "lora.hpp"
 #include "paged.hpp"
 
 #include <algorithm>
@@ -68,57 +67,6 @@ hipError_t launch_paged_attn(const PagedAttnParams& in, bool f16, int cus, hipSt
     else QORA_PAGED_W(64, false);
 #undef QORA_PAGED_W
 #undef QORA_PAGED
-    return hipGetLastError();
-}
-
-// K slices of the adapters' first step: enough workgroups for two a CU, of at least 512
-// rows (four waves of 128), and at most eight, which the second step adds up.
-void lora_shape(LoraParams* p, int cus) {
-    const uint32_t rb = (p->rows + 15u) / 16u;
-    p->slots = rb <= 4u ? 16u : 4u;
-    const uint32_t want = (2u * (uint32_t)std::max(1, cus) + rb * p->slots - 1u) / (rb * p->slots);
-    uint32_t nz = std::max(1u, std::min({want, (p->k + 511u) / 512u, kLoraSlices}));
-    p->kper = ((p->k + nz - 1u) / nz + 31u) / 32u * 32u;
-    p->nz = (p->k + p->kper - 1u) / p->kper;
-}
-
-static bool lora_ok(const LoraParams& p) {
-    return p.rows > 0 && p.k % 32 == 0 && p.n % 32 == 0 && p.kper % 32 == 0 && p.kper > 0 && p.slots > 0 &&
-           (uint64_t)p.nz * p.kper >= p.k && (uint64_t)(p.nz - 1u) * p.kper < p.k;
-}
-
-hipError_t launch_lora_shrink(const LoraParams& p, hipStream_t stream) {
-    const uint32_t rb = (p.rows + 15u) / 16u;
-    if (!lora_ok(p) || rb > 65535u) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(lora_shrink_kernel, dim3(p.slots, p.nz, rb), dim3(256), 0, stream, p);
-    return hipGetLastError();
-}
-
-hipError_t launch_lora_gemm_small(int fmt, const PfSmallParams& q, const LoraParams& p, hipStream_t stream) {
-    const uint32_t rb = (p.rows + 15u) / 16u, nx = (q.n + 127u) / 128u;
-    if (!lora_ok(p) || q.T != p.rows || q.k != p.k || q.n != p.n || !pf_small_ok(q)) return hipErrorInvalidValue;
-    const uint32_t ns = p.slots * p.nz * rb;
-    const dim3 grid(ns + nx * q.splits);
-#define QORA_LORA_SMALL(TM_)                                                                                        \
-    do {                                                                                                            \
-        if (fmt == FMT_Q4) hipLaunchKernelGGL((lora_gemm_small_kernel<TM_, true>), grid, dim3(256), 0, stream, q, p, ns, nx); \
-        else hipLaunchKernelGGL((lora_gemm_small_kernel<TM_, false>), grid, dim3(256), 0, stream, q, p, ns, nx);     \
-    } while (0)
-    if (q.T <= 16u) QORA_LORA_SMALL(1);
-    else if (q.T <= 32u) QORA_LORA_SMALL(2);
-    else QORA_LORA_SMALL(4);
-#undef QORA_LORA_SMALL
-    return hipGetLastError();
-}
-
-// Up to 64 rows the waves take the adapters in turn (lora_expand_kernel<true>).
-hipError_t launch_lora_expand(const LoraParams& p, const float* part, uint32_t splits, hipStream_t stream) {
-    const uint32_t rb = (p.rows + 15u) / 16u;
-    if (!lora_ok(p) || rb > 65535u || (splits > 1u && (!part || p.rows > kPfSmallT))) return hipErrorInvalidValue;
-    if (p.rows <= kPfSmallT)
-        hipLaunchKernelGGL((lora_expand_kernel<true>), dim3(p.n / 32u, rb), dim3(256), 0, stream, p, part, splits);
-    else
-        hipLaunchKernelGGL((lora_expand_kernel<false>), dim3((p.n + 255u) / 256u, rb), dim3(256), 0, stream, p, part, splits);
     return hipGetLastError();
 }
 
