@@ -2804,7 +2804,7 @@ extern "C" int qora_hip_paged_attn_prepare(qora_hip_ctx* c, uint32_t max_rows, u
         const uint32_t G = num_heads / num_kv_heads;
         const uint64_t items = paged_attn_items(max_rows, max_seqs, G, num_kv_heads, c->cus);
         const uint64_t cb = al256(items * sizeof(uint32_t));
-        if (items > 0x7FFFFFFFull) return fail(c, QORA_HIP_E_INVALID, "bad row or sequence count");
+        if (items > kPgMaxItems) return fail(c, QORA_HIP_E_INVALID, "more rows and sequences than one call can take");
         c->pattns.reserve(c->pattns.size() + 1);
         DeviceGuard dev(c->device);
         HIP_TRY(c, dev.err);

@@ -197,6 +197,18 @@ __device__ __forceinline__ PagedSeqPlan paged_seq_plan(const PagedAttnParams& p,
     return q;
 }
 
+// Inclusive sum over the wave's lanes, by DPP: within rows of 16, then row 0's and 2's last lane into the
+// next row, then lane 31's into the upper half.
+__device__ __forceinline__ uint32_t pg_scan(uint32_t v) {
+    v += dpp_u32<0x111>(v);    // row_shr:1 (lanes without a source add 0)
+    v += dpp_u32<0x112>(v);
+    v += dpp_u32<0x114>(v);
+    v += dpp_u32<0x118>(v);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);   // row_bcast:15 into rows 1 and 3
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);   // row_bcast:31 into rows 2 and 3
+    return v;
+}
+
 // The item of number `item`; false if there is none. All 64 lanes take part,
 // and every wave of the grid gets the same plan.
 __device__ bool paged_item(const PagedAttnParams& p, uint32_t item, PagedItem* it) {
@@ -215,20 +227,15 @@ __device__ bool paged_item(const PagedAttnParams& p, uint32_t item, PagedItem* i
         const float per_f = ceilf(share / (q.narrow ? p.narrow_cost : p.wide_cost));
         const uint32_t per = (uint32_t)fminf(fmaxf(per_f, 1.f), 1e9f);
         const uint32_t chunks = max((q.steps + per - 1u) / per, 1u);
-        const uint64_t mine = (uint64_t)p.g.KVH * q.tiles * chunks;
-        uint64_t sum = mine;                                  // inclusive scan
-#pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-            const uint64_t v = __shfl_up((unsigned long long)sum, o, kWave);
-            if (lane >= (uint32_t)o) sum += v;
-        }
+        // (more than any grid has: such a sequence is left out below, and so is what follows it)
+        const uint32_t mine = (uint32_t)min((uint64_t)p.g.KVH * q.tiles * chunks, (uint64_t)kPgMaxItems);
+        const uint32_t sum = pg_scan(mine);
         const uint64_t end = base + sum, begin = end - mine;
         const uint64_t hit = __ballot(item >= begin && item < end);
         if (hit) {
             const int w = __builtin_ctzll(hit);
             auto u = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, w); };
-            const uint64_t b0 = (uint64_t)u((uint32_t)begin) | ((uint64_t)u((uint32_t)(begin >> 32)) << 32);
-            const uint64_t e0 = (uint64_t)u((uint32_t)end) | ((uint64_t)u((uint32_t)(end >> 32)) << 32);
+            const uint64_t e0 = base + u(sum), b0 = e0 - u(mine);
             // row offsets that are none can ask for more items than the grid has: all of such a sequence is left out
             if (e0 > gridDim.x) return false;
             it->s = b + (uint32_t)w;
@@ -249,8 +256,7 @@ __device__ bool paged_item(const PagedAttnParams& p, uint32_t item, PagedItem* i
             it->first = (uint32_t)b0 + it->tile * p.g.KVH + it->kvh;
             return true;
         }
-        base += (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)sum, kWave - 1) |
-                ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(sum >> 32), kWave - 1) << 32);
+        base += (uint32_t)__builtin_amdgcn_readlane((int)sum, kWave - 1);
         if (base > item) return false;
     }
     return false;
@@ -692,25 +698,39 @@ __device__ __forceinline__ void paged_narrow(const PagedAttnParams& p, const Pag
         }
         if (!paged_arrive(p.count + it.first, it.chunks, shared)) return;
         if (row >= M) return;
+        // eight states in flight at a time, with a running maximum
+        constexpr uint32_t B = 8;
         float mx = -INFINITY;
-        for (uint32_t c = 0; c < it.chunks; ++c) mx = fmaxf(mx, pg_get2(state(c) + 16u * HD + 2u * row).x);
-        const float mf = mx == -INFINITY ? 0.f : mx;
         L0 = 0.f;
 #pragma unroll
         for (int d = 0; d < DL; ++d) acc[d] = 0.f;
-#pragma unroll 4
-        for (uint32_t c = 0; c < it.chunks; ++c) {
-            const float* b = state(c);
-            const float2 ml = pg_get2(b + 16u * HD + 2u * row);
-            float2 x[DL / 2];
+        for (uint32_t c0 = 0; c0 < it.chunks; c0 += B) {
+            float2 ml[B], x[B][DL / 2];
 #pragma unroll
-            for (int i = 0; i < DL / 2; ++i) x[i] = pg_get2(b + row * HD + d0 + 2 * i);
-            const float f = __builtin_amdgcn_exp2f(ml.x - mf);
-            L0 = fmaf(f, ml.y, L0);
+            for (uint32_t c = 0; c < B; ++c) {
+                const float* b = state(min(c0 + c, it.chunks - 1u));
+                ml[c] = pg_get2(b + 16u * HD + 2u * row);
 #pragma unroll
-            for (int i = 0; i < DL / 2; ++i) {
-                acc[2 * i] = fmaf(f, x[i].x, acc[2 * i]);
-                acc[2 * i + 1] = fmaf(f, x[i].y, acc[2 * i + 1]);
+                for (int i = 0; i < DL / 2; ++i) x[c][i] = pg_get2(b + row * HD + d0 + 2 * i);
+            }
+            float mn = mx;
+#pragma unroll
+            for (uint32_t c = 0; c < B; ++c) mn = fmaxf(mn, ml[c].x);
+            const float mf = mn == -INFINITY ? 0.f : mn, g0 = __builtin_amdgcn_exp2f(mx - mf);
+            mx = mn;
+            L0 *= g0;
+#pragma unroll
+            for (int d = 0; d < DL; ++d) acc[d] *= g0;
+#pragma unroll
+            for (uint32_t c = 0; c < B; ++c) {
+                if (c0 + c >= it.chunks) break;
+                const float f = __builtin_amdgcn_exp2f(ml[c].x - mf);
+                L0 = fmaf(f, ml[c].y, L0);
+#pragma unroll
+                for (int i = 0; i < DL / 2; ++i) {
+                    acc[2 * i] = fmaf(f, x[c][i].x, acc[2 * i]);
+                    acc[2 * i + 1] = fmaf(f, x[c][i].y, acc[2 * i + 1]);
+                }
             }
         }
     }
@@ -1126,9 +1146,8 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
         }
         if (!paged_arrive(p.count + it.first, lives, shared)) return;
         if (!wave_on) return;
+        // a state at a time (its loads together), with a running maximum
         float mx = -INFINITY;
-        for (uint32_t c = 0; c < lives; ++c) mx = fmaxf(mx, pg_get2(state(c) + kPgWideRows * HD + (wave * kWave + lane) * 2u).x);
-        const float mf = mx == -INFINITY ? 0.f : mx;
         l = 0.f;
 #pragma unroll
         for (int d = 0; d < OD; ++d)
@@ -1137,23 +1156,26 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
         for (uint32_t c = 0; c < lives; ++c) {
             const float* b = state(c);
             const float2 ml = pg_get2(b + kPgWideRows * HD + (wave * kWave + lane) * 2u);
-            const float f = __builtin_amdgcn_exp2f(ml.x - mf);
-            l = fmaf(f, ml.y, l);
+            float2 x[OD][8];
 #pragma unroll
-            for (int d = 0; d < OD; ++d) {
-                float2 x[8];
+            for (int d = 0; d < OD; ++d)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const float* y = b + ((wave * NJ + 4u * d + q) * kWave + lane) * 4u;
-                    x[2 * q] = pg_get2(y);
-                    x[2 * q + 1] = pg_get2(y + 2);
+                    x[d][2 * q] = pg_get2(y);
+                    x[d][2 * q + 1] = pg_get2(y + 2);
                 }
+            const float mn = fmaxf(mx, ml.x), mf = mn == -INFINITY ? 0.f : mn;
+            const float f0 = __builtin_amdgcn_exp2f(mx - mf), f = __builtin_amdgcn_exp2f(ml.x - mf);
+            mx = mn;
+            l = fmaf(f, ml.y, l * f0);
+#pragma unroll
+            for (int d = 0; d < OD; ++d)
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
-                    o[d][2 * q] = fmaf(f, x[q].x, o[d][2 * q]);
-                    o[d][2 * q + 1] = fmaf(f, x[q].y, o[d][2 * q + 1]);
+                    o[d][2 * q] = fmaf(f, x[d][q].x, o[d][2 * q] * f0);
+                    o[d][2 * q + 1] = fmaf(f, x[d][q].y, o[d][2 * q + 1] * f0);
                 }
-            }
         }
     }
     if (!wave_on || wave * 32u + li >= nrow) return;

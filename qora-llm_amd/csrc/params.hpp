@@ -431,6 +431,9 @@ struct PagedAppendParams {
     uint32_t units;            // 4-dim units of a row
 };
 
+// Most items (workgroups) of a paged attention call.
+constexpr uint32_t kPgMaxItems = 1u << 24;
+
 struct PagedAttnParams {
     PagedParams g;
     const float* q;

@@ -54,7 +54,7 @@ hipError_t launch_paged_attn(const PagedAttnParams& in, bool f16, int cus, hipSt
     p.least = 2.f;
     p.part_floats = pg_part_floats(HD, wide);
     const uint64_t items = paged_attn_items(p.g.rows, p.g.seqs, p.G, p.g.KVH, cus);
-    if (items > 0x7FFFFFFFull) return hipErrorInvalidValue;
+    if (items > kPgMaxItems) return hipErrorInvalidValue;
     const dim3 grid((uint32_t)items), block(256);
 #define QORA_PAGED(HD_, F_, W_) hipLaunchKernelGGL((paged_attn_kernel<HD_, F_, W_>), grid, block, 0, stream, p)
 #define QORA_PAGED_W(HD_, F_) \
