@@ -308,7 +308,7 @@ int qora_hip_argmax(qora_hip_ctx* ctx, const float* logits, uint64_t n, int32_t*
  * values starts at element page * page_stride + head * head_stride + slot *
  * slot_stride of k and of v. Rows may lie in any order of the three but not
  * over each other, and each starts on 16 bytes (E_INVALID otherwise); k and v
- * span at most 64 GiB each.
+ * span at most 64 GiB each and share no memory.
  * head_dim: a multiple of 8, at most 128. */
 typedef struct {
     void* k;
@@ -342,7 +342,8 @@ typedef struct {
  * floats apart (the three may be parts of one q|k|v row). q and k are rotated
  * with row `position` of cos_t, sin_t [rope_positions][half_dim] (half_dim 0:
  * not rotated); q goes to q_out, rows q_out_stride floats apart, which may be
- * q itself with the same stride; q and q_out both NULL: keys and values only.
+ * q itself with the same stride and otherwise may share no memory with q, k or
+ * v (E_INVALID); q and q_out both NULL: keys and values only.
  * A row whose position has no page or no row of the tables is skipped: q_out
  * and the cache stay as they were. Row pointers and strides are multiples of
  * 16 bytes. Two rows of one position and sequence page race. */
@@ -360,7 +361,8 @@ int qora_hip_paged_append(qora_hip_ctx* ctx, const qora_paged_kv* kv, const qora
  * out_stride floats apart; out may be q with the same stride, and may not
  * overlap it otherwise.
  * prepare allocates the workspace of calls of up to max_rows rows and max_seqs
- * sequences; release frees it (both refused during capture). Calls with one id,
+ * sequences; release frees it (both refused during capture), and with it ends
+ * the use of graphs that recorded a call. Calls with one id,
  * graph replays included, use its workspace and must run one behind the
  * other; work on several streams takes an id for each. */
 int qora_hip_paged_attn_prepare(qora_hip_ctx* ctx, uint32_t max_rows, uint32_t max_seqs, uint32_t num_heads,
@@ -384,9 +386,12 @@ typedef struct {
  * array of `rows` ids); an id outside 0 .. count - 1 means no adapter.
  * lora_upload packs `count` adapters (1 .. 65536) of [k][n] projections once
  * and allocates the workspace of calls of up to max_rows rows; lora_release
- * frees both (refused during capture). The weight's k and n must be the
- * adapters', n a multiple of 32 as in every upload. Calls with one lora id, and qora_hip_gemm's
- * scratch in the context, as there: one behind the other. y may be x. */
+ * frees both (refused during capture), and with them ends the use of graphs
+ * that recorded a call. The weight's k and n must be the adapters', both
+ * multiples of 32. Calls with one lora id use its workspace, and all use
+ * qora_hip_gemm's scratch in the context: they must run one behind the other,
+ * graph replays included; work on several streams takes a context for each.
+ * y may be x. */
 int qora_hip_lora_upload(qora_hip_ctx* ctx, const qora_lora_adapter* adapters, uint32_t count, uint64_t k, uint64_t n,
                          uint32_t max_rows, uint32_t* lora_id);
 int qora_hip_lora_release(qora_hip_ctx* ctx, uint32_t lora_id);

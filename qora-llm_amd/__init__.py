@@ -397,7 +397,11 @@ class HipContext:
         if rc != QORA_HIP_OK:
             raise QoraHipError(rc, f"qora_hip_create(device={device}) failed (no usable HIP device?)")
         self.h = h.value
-        self._paged_heads = {}     # paged attention id -> query heads (its default row stride)
+        # (the calls of every layer of a step: looked up once)
+        self._paged_append = self.lib.qora_hip_paged_append
+        self._paged_attn = self.lib.qora_hip_paged_attn_run
+        self._gemm_lora = self.lib.qora_hip_gemm_lora
+        self._paged_row = {}       # paged attention id -> floats of a row of q (its default stride)
 
     def check(self, rc: int, what: str = "") -> None:
         if rc != QORA_HIP_OK:
@@ -511,10 +515,12 @@ class HipContext:
         """Rotates the batch's q and k rows and stores k and v in the paged cache
         (device addresses; `stride` floats between rows of q, and of k and v unless
         given; q_out's rows are num_heads * head_dim apart unless given)."""
-        self.check(self.lib.qora_hip_paged_append(
-            self.h, ctypes.byref(kv), ctypes.byref(batch), num_heads, q or None, stride, k, k_stride or stride, v,
-            v_stride or stride, q_out or None, q_out_stride or num_heads * kv.head_dim, cos or None, sin or None,
-            half_dim, rope_positions, stream or None), "paged_append")
+        rc = self._paged_append(
+            self.h, ctypes.byref(kv), ctypes.byref(batch), num_heads, q, stride, k, k_stride or stride, v,
+            v_stride or stride, q_out, q_out_stride or num_heads * kv.head_dim, cos, sin, half_dim, rope_positions,
+            stream)
+        if rc:
+            self.check(rc, "paged_append")
 
     def paged_attn_prepare(self, max_rows: int, max_seqs: int, num_heads: int, num_kv_heads: int,
                            head_dim: int) -> int:
@@ -522,17 +528,18 @@ class HipContext:
         aid = ctypes.c_uint32()
         self.check(self.lib.qora_hip_paged_attn_prepare(self.h, max_rows, max_seqs, num_heads, num_kv_heads, head_dim,
                                                         ctypes.byref(aid)), "paged_attn_prepare")
-        self._paged_heads[aid.value] = num_heads
+        self._paged_row[aid.value] = num_heads * head_dim
         return aid.value
 
     def paged_attn_run(self, attn_id: int, kv: "PagedKV", batch: "PagedBatch", q: int, out: int, q_stride: int = 0,
                        out_stride: int = 0, stream: int = 0) -> None:
         """Causal attention of the batch's rows over the paged cache (device
         addresses; rows num_heads * head_dim floats apart unless given)."""
-        row = self._paged_heads.get(attn_id, 0) * kv.head_dim
-        self.check(self.lib.qora_hip_paged_attn_run(self.h, attn_id, ctypes.byref(kv), ctypes.byref(batch), q,
-                                                    q_stride or row, out, out_stride or row, stream or None),
-                   "paged_attn_run")
+        row = self._paged_row.get(attn_id, 0)
+        rc = self._paged_attn(self.h, attn_id, ctypes.byref(kv), ctypes.byref(batch), q, q_stride or row, out,
+                              out_stride or row, stream)
+        if rc:
+            self.check(rc, "paged_attn_run")
 
     def paged_attn_release(self, attn_id: int) -> None:
         self.check(self.lib.qora_hip_paged_attn_release(self.h, attn_id), "paged_attn_release")
@@ -559,8 +566,9 @@ class HipContext:
 
     def gemm_lora(self, wid: int, lora_id: int, x: int, y: int, rows: int, row_adapter: int, stream: int = 0) -> None:
         """y = x . W plus each row's own adapter (device addresses)."""
-        self.check(self.lib.qora_hip_gemm_lora(self.h, wid, lora_id, x, y, rows, row_adapter, stream or None),
-                   "gemm_lora")
+        rc = self._gemm_lora(self.h, wid, lora_id, x, y, rows, row_adapter, stream)
+        if rc:
+            self.check(rc, "gemm_lora")
 
     def weight_ptrs(self, wid: int):
         a, b = ctypes.c_void_p(), ctypes.c_void_p()

@@ -2719,9 +2719,6 @@ PagedParams paged_params(const qora_paged_kv* kv, const qora_paged_batch* b) {
     return g;
 }
 
-// Bytes from the first to the last element of `rows` rows.
-uint64_t rows_bytes(uint64_t rows, uint64_t ld, uint64_t width) { return rows ? ((rows - 1) * ld + width) * 4 : 0; }
-
 // No exception leaves a C entry: what the host's own containers throw (no
 // memory) is reported as such.
 template <typename F>
@@ -2758,10 +2755,13 @@ extern "C" int qora_hip_paged_append(qora_hip_ctx* c, const qora_paged_kv* kv, c
         if (!e) e = paged_rows_error(k, k_stride, kv->num_kv_heads, hd);
         if (!e) e = paged_rows_error(v, v_stride, kv->num_kv_heads, hd);
         if (e) return fail(c, QORA_HIP_E_INVALID, e);
-        if (q && !(q == q_out && q_stride == q_out_stride) &&
-            overlap(q, rows_bytes(batch->rows, q_stride, (uint64_t)num_heads * hd), q_out,
-                    rows_bytes(batch->rows, q_out_stride, (uint64_t)num_heads * hd)))
-            return fail(c, QORA_HIP_E_INVALID, "q_out overlaps q");
+        const uint64_t qw = (uint64_t)num_heads * hd;
+        const uint64_t kw = (uint64_t)kv->num_kv_heads * hd;
+        const uint64_t n = batch->rows;
+        if (q && ((!(q == q_out && q_stride == q_out_stride) && paged_rows_meet(q, q_stride, qw, q_out, q_out_stride, qw, n)) ||
+                  paged_rows_meet(q_out, q_out_stride, qw, k, k_stride, kw, n) ||
+                  paged_rows_meet(q_out, q_out_stride, qw, v, v_stride, kw, n)))
+            return fail(c, QORA_HIP_E_INVALID, "q_out overlaps q, k or v");
         PagedAppendParams p{};
         p.g = paged_params(kv, batch);
         p.q = q;
@@ -2847,8 +2847,7 @@ extern "C" int qora_hip_paged_attn_run(qora_hip_ctx* c, uint32_t attn_id, const 
         if (!e) e = paged_rows_error(out, out_stride, w.H, w.hd);
         if (e) return fail(c, QORA_HIP_E_INVALID, e);
         const uint64_t width = (uint64_t)w.H * w.hd;
-        if (!(q == out && q_stride == out_stride) &&
-            overlap(q, rows_bytes(batch->rows, q_stride, width), out, rows_bytes(batch->rows, out_stride, width)))
+        if (!(q == out && q_stride == out_stride) && paged_rows_meet(q, q_stride, width, out, out_stride, width, batch->rows))
             return fail(c, QORA_HIP_E_INVALID, "out overlaps q");
         PagedAttnParams p{};
         p.g = paged_params(kv, batch);
@@ -2931,11 +2930,15 @@ extern "C" int qora_hip_lora_upload(qora_hip_ctx* c, const qora_lora_adapter* ad
                 const uint32_t r = ad[i].rank;
                 const uint32_t rp = (r + 15u) & ~15u;
                 host.assign((size_t)rp * (k + n), 0);
-                for (uint64_t j = 0; j < k; ++j)
-                    for (uint32_t x = 0; x < r; ++x) host[x * k + j] = ad[i].a[j * r + x];
-                uint16_t* bt = host.data() + (size_t)rp * k;
-                for (uint32_t x = 0; x < r; ++x)
-                    for (uint64_t j = 0; j < n; ++j) bt[j * rp + x] = ad[i].b[x * n + j];
+                // (32 x 32 pieces: both sides' lines stay in the cache)
+                auto transpose = [](const uint16_t* in, uint64_t rows, uint64_t cols, uint16_t* out, uint64_t ld) {
+                    for (uint64_t i0 = 0; i0 < rows; i0 += 32)
+                        for (uint64_t j0 = 0; j0 < cols; j0 += 32)
+                            for (uint64_t j = j0; j < std::min(cols, j0 + 32); ++j)
+                                for (uint64_t i2 = i0; i2 < std::min(rows, i0 + 32); ++i2) out[j * ld + i2] = in[i2 * cols + j];
+                };
+                transpose(ad[i].a, k, r, host.data(), k);
+                transpose(ad[i].b, r, n, host.data() + (size_t)rp * k, rp);
                 uint8_t* d = (uint8_t*)s.mem + at;
                 entries[i] = LoraEntry{(const uint16_t*)d, (const uint16_t*)(d + 2u * rp * k), rp, ad[i].scale};
                 e = hipMemcpy(d, host.data(), host.size() * 2, hipMemcpyHostToDevice);

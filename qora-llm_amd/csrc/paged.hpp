@@ -225,7 +225,7 @@ __device__ bool paged_item(const PagedAttnParams& p, uint32_t item, PagedItem* i
     for (uint32_t b = 0; b < seqs; b += kWave) {
         const PagedSeqPlan q = b == 0 ? q0 : paged_seq_plan(p, b + lane);
         const float per_f = ceilf(share / (q.narrow ? p.narrow_cost : p.wide_cost));
-        const uint32_t per = (uint32_t)fminf(fmaxf(per_f, 1.f), 1e9f);
+        const uint32_t per = min((uint32_t)fminf(fmaxf(per_f, 1.f), 1e9f), max(q.steps, 1u));
         const uint32_t chunks = max((q.steps + per - 1u) / per, 1u);
         // (more than any grid has: such a sequence is left out below, and so is what follows it)
         const uint32_t mine = (uint32_t)min((uint64_t)p.g.KVH * q.tiles * chunks, (uint64_t)kPgMaxItems);
@@ -783,7 +783,7 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
     // keys that the tile's last row sees bound its chunks
     const int64_t last_pos = it.pos0 + (int64_t)((r0 + nrow - 1u) / p.G);
     const uint32_t klen = (uint32_t)max((int64_t)0, min((int64_t)it.len, last_pos + 1));
-    const uint32_t ckeys = it.per > 0x7FFFFFFFu / KT ? 0x7FFFFFFFu / KT * KT : it.per * KT;
+    const uint32_t ckeys = it.per * KT;                      // (at most the sequence's keys and a step: 32 bits)
     const uint32_t lives = max(1u, (klen + ckeys - 1u) / ckeys);
     if (it.chunk >= lives) return;
     const uint32_t kbeg = it.chunk * ckeys, kend = min(klen, kbeg + ckeys);
@@ -898,7 +898,8 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
 
     uint64_t live, live1 = 0;
     uint32_t unit = unit_of(kbeg, page, &live);
-    load_tile(unit, 0);
+    // (nothing may be on its way to LDS when the workgroup ends: a tile of rows at negative positions only has no keys)
+    if (kbeg < kend) load_tile(unit, 0);
     uint32_t buf = 0;
     // LDS places: K piece 2 st + h of key li is at kl0 ^ 32 st; the V piece of dim tile d, keys 8 j .. (with the
     // lane's part of them) at vl0 ^ (64 d + 32 j), rows further by whole rows

@@ -96,8 +96,22 @@ inline const char* paged_batch_error(const qora_paged_kv* kv, const qora_paged_b
 inline const char* paged_rows_error(const void* p, uint64_t ld, uint64_t heads, uint32_t hd) {
     if (!p) return "null argument";
     if (((uintptr_t)p) % 16 != 0 || ld % 4 != 0) return "rows must be 16-byte aligned";
-    if (ld < heads * hd || ld >= (1ull << 40)) return "row stride does not hold the heads";
+    if (ld < heads * hd || ld >= (1ull << 30)) return "row stride does not hold the heads";
     return nullptr;
+}
+
+// Whether two arrays of `rows` rows, ld floats apart and w floats wide, share memory. Rows of the same stride
+// may lie between each other (the parts of a q|k|v row).
+inline bool paged_rows_meet(const void* a, uint64_t lda, uint64_t wa, const void* b, uint64_t ldb, uint64_t wb,
+                            uint64_t rows) {
+    if (rows == 0) return false;
+    const uint64_t x = (uint64_t)(uintptr_t)a, y = (uint64_t)(uintptr_t)b;
+    const uint64_t xe = x + ((rows - 1) * lda + wa) * 4, ye = y + ((rows - 1) * ldb + wb) * 4;
+    if (xe <= y || ye <= x) return false;
+    if (lda != ldb || (y - x) % 4 != 0) return true;
+    // b's first column after a's, modulo the stride
+    const uint64_t d = y >= x ? (y - x) / 4 % lda : (lda - (x - y) / 4 % lda) % lda;
+    return d < wa || d + wb > lda;
 }
 
 }  // namespace qora

@@ -124,6 +124,29 @@ int main() {
     CHECK(!paged_rows_error(mem, 16, 2, 8) && paged_rows_error(nullptr, 16, 2, 8) && paged_rows_error(mem, 12, 2, 8) &&
           paged_rows_error(mem, 18, 2, 8) && paged_rows_error((char*)mem + 8, 16, 2, 8) &&
           paged_rows_error(mem, 1ull << 40, 2, 8));
+    // rows against a brute-force look for a shared float
+    static float f[4096];
+    int meet = 0;
+    for (int i = 0; i < 20000; ++i) {
+        const uint64_t wa = 1 + rnd(12), wb = 1 + rnd(12), rows = 1 + rnd(6);
+        const uint64_t lda = wa + rnd(16), ldb = rnd(2) ? lda : wb + rnd(16);
+        if (ldb < wb) continue;
+        const float *a = f + 1000 + rnd(80), *b = f + 1000 + rnd(80);
+        bool shared = false;
+        for (uint64_t r = 0; r < rows; ++r)
+            for (uint64_t q = 0; q < rows; ++q) {
+                const float *x = a + r * lda, *y = b + q * ldb;
+                shared = shared || (x < y + wb && y < x + wa);
+            }
+        const bool said = paged_rows_meet(a, lda, wa, b, ldb, wb, rows);
+        CHECK(said || !shared);                      // (what meets in no row may be refused where the strides differ)
+        if (lda == ldb && said && !shared) ++meet;   // or wraps around the end of the last row
+    }
+    CHECK(meet < 400);
+    float qkv[3][48];
+    CHECK(!paged_rows_meet(qkv[0], 48, 16, qkv[0] + 16, 48, 16, 3) && !paged_rows_meet(qkv[0] + 32, 48, 16, qkv[0], 48, 16, 3));
+    CHECK(paged_rows_meet(qkv[0], 48, 16, qkv[0] + 15, 48, 16, 3) && paged_rows_meet(qkv[0], 48, 16, qkv[0], 48, 16, 3));
+    CHECK(paged_rows_meet(qkv[0], 16, 16, qkv[0] + 16, 48, 16, 3) && !paged_rows_meet(qkv[0], 48, 16, qkv[2] + 16, 48, 16, 0));
     std::printf(fails ? "%d failed\n" : "all cases held\n", fails);
     return fails != 0;
 }

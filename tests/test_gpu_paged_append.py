@@ -202,7 +202,8 @@ def test_append_refusals(ctx, pkg):
         assert call() == pkg.QORA_HIP_OK
         bad = [dict(kv=None), dict(b=None), dict(q=None), dict(o=None), dict(k=None), dict(v=None), dict(c=None),
                dict(s=None), dict(half=33), dict(n=0), dict(H=0), dict(qs=H * hd - 4), dict(ks=KVH * hd - 4),
-               dict(qs=row + 1), dict(q=p + 4), dict(o=p + 16, os=row), dict(os=H * hd - 4)]
+               dict(qs=row + 1), dict(q=p + 4), dict(o=p + 16, os=row), dict(os=H * hd - 4),
+               dict(o=p + 4 * H * hd, os=row), dict(o=p + 4 * row - 16 * hd, os=row), dict(qs=2 ** 30)]
         for ch in bad:
             assert call(**ch) == pkg.QORA_HIP_E_INVALID, ch
         # nothing to do is no error, whatever the row arrays are

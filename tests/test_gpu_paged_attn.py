@@ -102,7 +102,8 @@ def test_attention_by_the_most_rows(ctx, pkg, kv, max_new):
 def test_rows_that_see_nothing_are_zero(ctx, pkg, kv):
     """Lengths shorter than the new rows, lengths of 0 and below, and pages that are all outside the pool."""
     r = rng(6)
-    seqs = [(3, 0), (4, 2), (1, -7), (2, 5), (1, 3), (20, 11)]
+    # (the last two: tiles of 128 rows that see nothing, in front of work that follows)
+    seqs = [(3, 0), (4, 2), (1, -7), (2, 5), (1, 3), (20, 11), (40, 0), (90, 17)]
     batch, pool, q = _inputs(pkg, r, kv, "head", 4, 8, 2, 64, seqs, bad={(3, 0): -1, (3, 1): 10 ** 7, (4, 0): -2 ** 31})
     ref, tol = attention64(pool, batch, q, 8)
     with device(ctx) as d:
