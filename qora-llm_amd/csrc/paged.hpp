@@ -142,9 +142,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams p) 
 // state lives in its own lanes and its weights never leave them.
 // Numerics: the matrix cores take two-byte operands. Over a binary16 cache K and V
 // are exact, q (on a power-of-two scale of its row) and the weights (times 2^15)
-// are split into two binary16 parts; over a float32 cache every operand is split
-// into three bfloat16 parts by cutting its bits (exact: 3 x 8 = 24), and the six
-// products above 2^-24 are kept. Sums are float32.
+// are split into two binary16 parts (22 bits). Over a float32 cache narrow items split every
+// operand into three bfloat16 parts by cutting its bits (exact: 3 x 8 = 24) and keep the six
+// products above 2^-24, which cost nothing beside the loads; wide items, bound by the products,
+// split K and V into two binary16 parts too, on a power-of-two scale of each key's own, and keep
+// three products. Sums are float32.
 // ---------------------------------------------------------------------------
 typedef _Float16 pg_half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 pg_bf8 __attribute__((ext_vector_type(8)));
@@ -310,6 +312,9 @@ __device__ __forceinline__ float2 pg_get2(const float* p) {
     const pg_u64 v = __hip_atomic_load(reinterpret_cast<const pg_u64*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
+
+// A word of a vector by value (a bit cast of the element itself would read element 0).
+__device__ __forceinline__ uint32_t pg_word(const v4u32& x, int i) { return x[i]; }
 
 // Binary16 words / float32 words that are infinite or NaN.
 template <bool F16>
@@ -748,10 +753,10 @@ __device__ __forceinline__ void paged_narrow(const PagedAttnParams& p, const Pag
 // 8 j + 4 h + r, then O^T += V^T P^T with V^T from transposing LDS reads
 // (ds_read_b64_tr_b16: 4 keys x 16 dims of a row-major tile). Over a binary16 cache the tile
 // goes from the cache to LDS past the registers, one tile ahead, two buffers and one barrier
-// a tile; a float32 tile is loaded into registers a tile ahead and cut into its three parts
-// on the way to LDS. 16-byte pieces of an LDS row are permuted by the row so that neither the
+// a tile; a float32 tile is loaded into registers a tile ahead and split into two binary16 parts
+// a key on the way to LDS. 16-byte pieces of an LDS row are permuted by the row so that neither the
 // reads of 32 keys' pieces nor the transposing reads of 4 keys meet in a bank.
-// What bounds a chunk of 512 rows over 8192 keys is the matrix cores' two (six) products and
+// What bounds a chunk of 512 rows over 8192 keys is the matrix cores' two (three) products and
 // the softmax's vector instructions beside them, about as many cycles.
 template <int HD>
 __device__ __forceinline__ uint32_t pg_swz_k(uint32_t row) {
@@ -768,8 +773,7 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
     constexpr int KB = KT / 32;                              // 32-key score tiles
     constexpr int QS = HD / 16;                              // 16-deep steps of q.k
     constexpr int OD = HD / 32;                              // 32-dim output tiles
-    constexpr int NP = F16 ? 2 : 3;                          // parts of q and the weights
-    constexpr int KP = F16 ? 1 : 3;                          // parts of k and v
+    constexpr int KP = F16 ? 1 : 2;                          // parts of k and v (two of q and the weights)
     constexpr uint32_t ES = F16 ? 2u : 4u;
     constexpr uint32_t CPR = HD / 8;                         // 16-byte pieces of an LDS row
     constexpr uint32_t TB = KT * HD * 2u;                    // bytes of a tile part in LDS
@@ -804,7 +808,9 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
         return on ? paged_row_unit(p, it.kvh, page, key % g.page_size) : it.kvh * p.head_u;
     };
     const uint32_t kt0 = (uint32_t)(uintptr_t)(pg_lds_p)smem;   // binary16: [buffer]; float32: [part]
-    const uint32_t vt0 = kt0 + (F16 ? 2u : 3u) * TB;
+    const uint32_t vt0 = kt0 + 2u * TB;
+    float* const kexp = reinterpret_cast<float*>(smem + 4u * TB);   // float32: 2^e of each key's k, then e of its v
+    float* const vexp = kexp + KT;
     constexpr int NL = (int)(KT * HD * ES / 16u / 256u);     // 16-byte pieces of K (and V) a thread moves
     v4u32 kreg[F16 ? 1 : NL], vreg[F16 ? 1 : NL];
     auto load_tile = [&](uint32_t unit, uint32_t buf) {
@@ -830,7 +836,8 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
             }
         }
     };
-    auto store_tile = [&]() {                                // float32: three parts of four dims, 8 bytes each
+    // float32: a row's HD / 4 lanes share its exponent (of its largest finite value), then two parts of four dims
+    auto store_tile = [&]() {
         if constexpr (!F16) {
             const uint32_t ln = pg_fresh(lane);
 #pragma unroll
@@ -839,23 +846,35 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
                 const uint32_t row = (wave * NL + (uint32_t)j) * RW + ln / PR, c = ln % PR;
                 const uint32_t ak = kt0 + (row * CPR + ((c / 2u) ^ pg_swz_k<HD>(row))) * 16u + (c % 2u) * 8u;
                 const uint32_t av = vt0 + (row * CPR + ((c / 2u) ^ pg_swz_v<HD>(row))) * 16u + (c % 2u) * 8u;
-                uint32_t a[3], b[3];
-                pg_cut2(__uint_as_float(kreg[j][0]), __uint_as_float(kreg[j][1]), &a[0], &a[1], &a[2]);
-                pg_cut2(__uint_as_float(kreg[j][2]), __uint_as_float(kreg[j][3]), &b[0], &b[1], &b[2]);
+                auto put = [&](const v4u32& x, uint32_t at) {
+                    float amax = 0.f;
 #pragma unroll
-                for (uint32_t q = 0; q < 3; ++q)
-                    *reinterpret_cast<__attribute__((address_space(3))) v2u32*>(ak + q * TB) = v2u32{a[q], b[q]};
-                pg_cut2(__uint_as_float(vreg[j][0]), __uint_as_float(vreg[j][1]), &a[0], &a[1], &a[2]);
-                pg_cut2(__uint_as_float(vreg[j][2]), __uint_as_float(vreg[j][3]), &b[0], &b[1], &b[2]);
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t u = x[i] & 0x7FFFFFFFu;
+                        amax = fmaxf(amax, u < 0x7F800000u ? __uint_as_float(u) : 0.f);
+                    }
+                    amax = group_max<PR>(amax);
+                    int e = 0;
+                    (void)frexpf(amax, &e);
+                    e = max(e - 15, -100);                   // (smaller rows: 2^-100 and its square stay in range)
+                    uint32_t a[2], b[2];
+                    pg_split2(ldexpf(__uint_as_float(pg_word(x, 0)), -e), ldexpf(__uint_as_float(pg_word(x, 1)), -e), &a[0], &a[1]);
+                    pg_split2(ldexpf(__uint_as_float(pg_word(x, 2)), -e), ldexpf(__uint_as_float(pg_word(x, 3)), -e), &b[0], &b[1]);
 #pragma unroll
-                for (uint32_t q = 0; q < 3; ++q)
-                    *reinterpret_cast<__attribute__((address_space(3))) v2u32*>(av + q * TB) = v2u32{a[q], b[q]};
+                    for (uint32_t q = 0; q < 2; ++q)
+                        *reinterpret_cast<__attribute__((address_space(3))) v2u32*>(at + q * TB) = v2u32{a[q], b[q]};
+                    return e;
+                };
+                const int ek = put(kreg[j], ak), ev = put(vreg[j], av);
+                if (c == 0) {
+                    kexp[row] = ldexpf(1.f, ek);
+                    vexp[row] = (float)ev;
+                }
             }
         }
     };
 
     int32_t page = page_of(kbeg), page1 = page_of(kbeg + KT);
-    // q: its two parts; over a float32 cache the values themselves (64 registers instead of 96), cut at each use
     v4u32 qp[2][QS];
     float qf = p.scale * 1.4426950408889634f;
     {
@@ -872,24 +891,25 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
             for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(qv[st][i]));
         }
         int e = 0;
-        if constexpr (F16) {
-            amax = fmaxf(amax, __shfl_xor(amax, 32, kWave));
-            (void)frexpf(amax, &e);
-            e -= 15;
-            qf *= ldexpf(1.f, e);
-        }
+        amax = fmaxf(amax, __shfl_xor(amax, 32, kWave));
+        (void)frexpf(amax, &e);
+        e = max(e - 15, -100);
+        qf *= ldexpf(1.f, e);
 #pragma unroll
         for (int st = 0; st < QS; ++st)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                uint32_t w[2] = {__float_as_uint(qv[st][2 * i]), __float_as_uint(qv[st][2 * i + 1])};
-                if constexpr (F16) pg_split2(ldexpf(qv[st][2 * i], -e), ldexpf(qv[st][2 * i + 1], -e), &w[0], &w[1]);
-#pragma unroll
-                for (int a = 0; a < 2; ++a) qp[a][st][i] = w[a];
+                uint32_t hi, lo;
+                pg_split2(ldexpf(qv[st][2 * i], -e), ldexpf(qv[st][2 * i + 1], -e), &hi, &lo);
+                qp[0][st][i] = hi;
+                qp[1][st][i] = lo;
             }
     }
-    constexpr float kBoost = F16 ? 15.f : 0.f;
-    float m = -INFINITY, l = 0.f;
+    // Weights go into the products times 2^15 (binary16's range). Over a float32 cache each key's values have an
+    // exponent of their own, which its weight takes on: 2^(score + e_v - top + 15), top the row's running maximum of
+    // score + e_v over the keys it sees, so that no key, however large, costs another its bits.
+    constexpr float kBoost = 15.f;
+    float m = -INFINITY, top = -INFINITY, l = 0.f;
     pg_f16 o[OD];
 #pragma unroll
     for (int d = 0; d < OD; ++d)
@@ -953,28 +973,26 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
 #pragma unroll
                 for (int q = 0; q < KP; ++q) kf[q][b] = pg_lds<v4u32>(at + q * TB);
             }
-            if constexpr (F16) {
+            auto mm = [&](const v4u32* k, const v4u32& q) {
 #pragma unroll
-                for (int a = 0; a < 2; ++a)
+                for (int b = 0; b < KB; ++b)
+                    sacc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(pg_half8, k[b]),
+                                                                     __builtin_bit_cast(pg_half8, q), sacc[b], 0, 0, 0);
+            };
+            mm(kf[0], qp[0][st]);
+            if constexpr (KP == 2) mm(kf[1], qp[0][st]);
+            mm(kf[0], qp[1][st]);
+        }
+        // float32: the keys' own scales, and their values' exponents
+        float ve[F16 ? 1 : 16];
+        const float qs = F16 ? qf : 1.f;
+        if constexpr (!F16) {
 #pragma unroll
-                    for (int b = 0; b < KB; ++b)
-                        sacc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(pg_half8, kf[0][b]),
-                                                                         __builtin_bit_cast(pg_half8, qp[a][st]), sacc[b], 0, 0, 0);
-            } else {
-                v4u32 qc[3];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t w[3];
-                    pg_cut2(__uint_as_float(pg_fresh(qp[0][st][i])), __uint_as_float(pg_fresh(qp[1][st][i])), &w[0], &w[1], &w[2]);
-#pragma unroll
-                    for (int a = 0; a < 3; ++a) qc[a][i] = w[a];
-                }
-#pragma unroll
-                for (int a = 2; a >= 0; --a)
-#pragma unroll
-                    for (int c = 2 - a; c >= 0; --c)
-                        sacc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pg_bf8, kf[a][0]),
-                                                                          __builtin_bit_cast(pg_bf8, qc[c]), sacc[0], 0, 0, 0);
+            for (int v = 0; v < 16; v += 4) {
+                const float4 ks = *reinterpret_cast<const float4*>(kexp + 2 * v + 4u * h);
+                const float4 vs = *reinterpret_cast<const float4*>(vexp + 2 * v + 4u * h);
+                sacc[0][v] *= ks.x * qf; sacc[0][v + 1] *= ks.y * qf; sacc[0][v + 2] *= ks.z * qf; sacc[0][v + 3] *= ks.w * qf;
+                ve[v] = vs.x; ve[v + 1] = vs.y; ve[v + 2] = vs.z; ve[v + 3] = vs.w;
             }
         }
         // ---- masks and running softmax of row li: keys 32 b + 8 (v / 4) + 4 h + v % 4 ----
@@ -1002,20 +1020,30 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
             for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sacc[b][v]);
         {
             const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-            mx = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])) * qf;
+            mx = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])) * qs;
         }
         const float mn = fmaxf(m, mx);
         const float mref = mn == -INFINITY ? 0.f : mn;
-        if (__ballot(mn > m)) {
-            const float f = __builtin_amdgcn_exp2f(m - mref);
-            l *= f;
+        float tn = mn;                                       // the weights' own maximum
+        if constexpr (!F16) {
+            float tx = sacc[0][0] + ve[0];
+#pragma unroll
+            for (int v = 1; v < 16; ++v) tx = fmaxf(tx, sacc[0][v] + ve[v]);
+            const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(tx), __float_as_uint(tx), false, false);
+            tn = fmaxf(top, fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])));
+        }
+        const float tref = tn == -INFINITY ? 0.f : tn;
+        if (__ballot(tn > top || mn > m)) {
+            const float f = __builtin_amdgcn_exp2f(top - tref);
+            l *= __builtin_amdgcn_exp2f(m - mref);
 #pragma unroll
             for (int d = 0; d < OD; ++d)
 #pragma unroll
                 for (int v = 0; v < 16; ++v) o[d][v] *= f;
         }
         m = mn;
-        const float shift = kBoost - mref;                   // weight 2^(score qf - mref + boost)
+        top = tn;
+        const float shift = kBoost - tref;                   // a weight on its values' scale: 2^(score qs + shift)
         // ---- values: keys nobody sees read as zero, and a key that only some of the rows see
         // must not meet the others' zero weights when its values are not finite ----
         const uint32_t vl = vt + pg_fresh(vl0);
@@ -1034,10 +1062,9 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
                         const v4u32 a = v_frag(vl, t4, d);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            // binary16: exponent of all ones; a cut float32's first part carries it
-                            const uint32_t x = (a[i / 2] >> (16 * (i % 2))) & 0xFFFFu;
-                            const uint32_t ex = F16 ? 0x7C00u : 0x7F80u;
-                            const uint64_t who = __ballot((x & ex) == ex);
+                            // (a float32's first part carries it)
+                            const uint32_t x = (a[i / 2] >> (16 * (i % 2))) & 0x7C00u;
+                            const uint64_t who = __ballot(x == 0x7C00u);
                             const uint32_t key = 16u * t4 + 8u * (i / 4) + i % 4;
                             if (who & 0xFFFFFFFFull) bad |= 1ull << key;
                             if (who >> 32) bad |= 1ull << (key + 4u);
@@ -1054,7 +1081,7 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
                     for (int b = 0; b < KB; ++b)
 #pragma unroll
                         for (int v = 0; v < 16; ++v) {
-                            const float e = __builtin_amdgcn_exp2f(fmaf(sacc[b][v], qf, sh));
+                            const float e = __builtin_amdgcn_exp2f(fmaf(sacc[b][v], qs, sh));
                             mine = (uint32_t)(16 * b + v) == want ? e : mine;
                         }
                     const float w = __shfl(mine, (int)(32u * ((key / 4u) % 2u) + li), kWave);
@@ -1073,20 +1100,27 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
                 }
             }
         }
-        v4u32 pp[NP][2 * KB];
+        v4u32 pp[2][2 * KB];
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
             float ls = 0.f;
 #pragma unroll
             for (int v = 0; v < 16; v += 2) {
-                const float e0 = __builtin_amdgcn_exp2f(fmaf(sacc[b][v], qf, shift));
-                const float e1 = __builtin_amdgcn_exp2f(fmaf(sacc[b][v + 1], qf, shift));
-                ls += e0 + e1;
-                uint32_t w[3];
-                if constexpr (F16) pg_split2(e0, e1, &w[0], &w[1]);
-                else pg_cut2(e0, e1, &w[0], &w[1], &w[2]);
+                float e[2];
 #pragma unroll
-                for (int a = 0; a < NP; ++a) pp[a][2 * b + v / 8][(v % 8) / 2] = w[a];
+                for (int i = 0; i < 2; ++i) {
+                    if constexpr (F16) {
+                        e[i] = __builtin_amdgcn_exp2f(fmaf(sacc[b][v + i], qs, shift));
+                        ls += e[i];
+                    } else {
+                        ls += __builtin_amdgcn_exp2f(sacc[b][v + i] - mref);
+                        e[i] = __builtin_amdgcn_exp2f(sacc[b][v + i] + ve[v + i] + shift);
+                    }
+                }
+                uint32_t hi, lo;
+                pg_split2(e[0], e[1], &hi, &lo);
+                pp[0][2 * b + v / 8][(v % 8) / 2] = hi;
+                pp[1][2 * b + v / 8][(v % 8) / 2] = lo;
             }
             l += ls;
         }
@@ -1108,21 +1142,23 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
                 v4u32 a[KP];
 #pragma unroll
                 for (int q = 0; q < KP; ++q) a[q] = v_frag(vl + q * TB, t4, d) & keep;
-                if constexpr (F16) {
-#pragma unroll
-                    for (int b = 0; b < 2; ++b)
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(pg_half8, a[0]),
-                                                                      __builtin_bit_cast(pg_half8, pp[b][t4]), o[d], 0, 0, 0);
-                } else {
-#pragma unroll
-                    for (int q = 2; q >= 0; --q)
-#pragma unroll
-                        for (int b = 2 - q; b >= 0; --b)
-                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pg_bf8, a[q]),
-                                                                           __builtin_bit_cast(pg_bf8, pp[b][t4]), o[d], 0, 0, 0);
-                }
+                auto mm = [&](const v4u32& v, const v4u32& w) {
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(pg_half8, v),
+                                                                  __builtin_bit_cast(pg_half8, w), o[d], 0, 0, 0);
+                };
+                mm(a[0], pp[0][t4]);
+                if constexpr (KP == 2) mm(a[1], pp[0][t4]);
+                mm(a[0], pp[1][t4]);
             }
         }
+    }
+    if constexpr (!F16) {
+        // from the values' scale to the weights' 2^(score - m)
+        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - kBoost - m);
+#pragma unroll
+        for (int d = 0; d < OD; ++d)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[d][v] *= f;
     }
     {
         const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
@@ -1198,7 +1234,7 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
 template <int HD, bool F16, bool WIDE>
 __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnParams p) {
     constexpr uint32_t kNarrowLds = (4u * 16u * (HD + 4u) + 128u) * 4u;
-    constexpr uint32_t kWideLds = (F16 ? 4u : 6u) * pg_wide_keys(F16) * HD * 2u;
+    constexpr uint32_t kWideLds = 4u * pg_wide_keys(F16) * HD * 2u + (F16 ? 0u : pg_wide_keys(F16) * 8u);
     __shared__ __align__(256) char smem[WIDE && kWideLds > kNarrowLds ? kWideLds : kNarrowLds];
     __shared__ uint32_t shared;
     PagedItem it;
