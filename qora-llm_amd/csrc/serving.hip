@@ -23,7 +23,9 @@ hipError_t launch_paged_append(const PagedAppendParams& in, bool f16, hipStream_
     return hipGetLastError();
 }
 
-// Items the work is cut into: twice the CUs, two workgroups on each.
+// Items the work is cut into: twice the CUs, two workgroups on each. (512 rows over 8192 keys, calls on one stream
+// / on three: 116 / 76 us; with half as many 125 / 72; 65535 positions 67 / 37.6 and 62 / 36.5; 4096 in f32
+// 51.6 / 23.1 and 52.2 / 24.3.)
 static uint32_t paged_target(int cus) { return 2u * (uint32_t)std::max(1, cus); }
 
 // Items beyond the target: every tile's last chunk may be a short one.
@@ -48,10 +50,14 @@ hipError_t launch_paged_attn(const PagedAttnParams& in, bool f16, int cus, hipSt
     const bool wide = paged_wide_rows(p.g.max_new, p.G);
     p.narrow_keys = pg_narrow_keys(f16);
     p.wide_keys = pg_wide_keys(f16);
-    p.narrow_cost = 2.f;
+    // A narrow step (128 binary16 keys of a row or two) takes a workgroup about as long as four wide ones (64 keys of
+    // 128 rows): one chunk beside 16 single tokens, calls on one stream / on three, 99.5 / 54.5 us at two, 90.9 / 52.4
+    // at four, 98.5 / 52.1 at six. No item is shorter than one narrow step or four wide ones: a state to store
+    // and join costs as much as that.
+    p.narrow_cost = 4.f;
     p.wide_cost = 1.f;
     p.target = (float)paged_target(cus);
-    p.least = 2.f;
+    p.least = 4.f;
     p.part_floats = pg_part_floats(HD, wide);
     const uint64_t items = paged_attn_items(p.g.rows, p.g.seqs, p.G, p.g.KVH, cus);
     if (items > kPgMaxItems) return hipErrorInvalidValue;
