@@ -313,6 +313,21 @@ __device__ __forceinline__ float2 pg_get2(const float* p) {
     return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
+// Largest of the values of each aligned group of N = 16 or 32 lanes, in every lane of it.
+template <int N>
+__device__ __forceinline__ uint32_t pg_group_max(uint32_t v) {
+    static_assert(N == 16 || N == 32, "16- or 32-lane groups");
+    v = max(v, dpp_u32<0xB1>(v));     // quad_perm [1,0,3,2]
+    v = max(v, dpp_u32<0x4E>(v));     // quad_perm [2,3,0,1]
+    v = max(v, dpp_u32<0x141>(v));    // row_half_mirror
+    v = max(v, dpp_u32<0x140>(v));    // row_mirror
+    if constexpr (N == 32) {
+        const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = max((uint32_t)a[0], (uint32_t)a[1]);
+    }
+    return v;
+}
+
 // A word of a vector by value (a bit cast of the element itself would read element 0).
 __device__ __forceinline__ uint32_t pg_word(const v4u32& x, int i) { return x[i]; }
 
@@ -847,16 +862,19 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
                 const uint32_t ak = kt0 + (row * CPR + ((c / 2u) ^ pg_swz_k<HD>(row))) * 16u + (c % 2u) * 8u;
                 const uint32_t av = vt0 + (row * CPR + ((c / 2u) ^ pg_swz_v<HD>(row))) * 16u + (c % 2u) * 8u;
                 auto put = [&](const v4u32& x, uint32_t at) {
-                    float amax = 0.f;
+                    // (magnitudes compare as integers; a row that holds a value that is not finite looks again without those)
+                    auto most = [&](uint32_t lim) {
+                        uint32_t u = 0;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t u = x[i] & 0x7FFFFFFFu;
-                        amax = fmaxf(amax, u < 0x7F800000u ? __uint_as_float(u) : 0.f);
-                    }
-                    amax = group_max<PR>(amax);
-                    int e = 0;
-                    (void)frexpf(amax, &e);
-                    e = max(e - 15, -100);                   // (smaller rows: 2^-100 and its square stay in range)
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t y = pg_word(x, i) & 0x7FFFFFFFu;
+                            u = max(u, y < lim ? y : 0u);
+                        }
+                        return pg_group_max<PR>(u);
+                    };
+                    uint32_t u = most(~0u);
+                    if (__ballot(u >= 0x7F800000u)) u = most(0x7F800000u);
+                    const int e = max((int)(u >> 23) - 141, -100);   // |v| 2^-e < 2^15 (smaller rows: 2^-100 stays in range)
                     uint32_t a[2], b[2];
                     pg_split2(ldexpf(__uint_as_float(pg_word(x, 0)), -e), ldexpf(__uint_as_float(pg_word(x, 1)), -e), &a[0], &a[1]);
                     pg_split2(ldexpf(__uint_as_float(pg_word(x, 2)), -e), ldexpf(__uint_as_float(pg_word(x, 3)), -e), &b[0], &b[1]);
@@ -1130,25 +1148,36 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
 #pragma unroll
         for (int t4 = 0; t4 < 2 * KB; ++t4) {
             v4u32 keep = {~0u, ~0u, ~0u, ~0u};
-            if (use != all) {
+            constexpr int DG = KP == 1 || OD == 1 ? OD : OD / 2;   // dim tiles whose pieces are in registers at a time
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t key = 16u * t4 + 8u * (i / 4) + i % 4;
-                    if (!((there >> key) & 1ull)) keep[i / 2] &= i % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+            for (int d0 = 0; d0 < OD; d0 += DG) {
+                v4u32 a[DG][KP];
+#pragma unroll
+                for (int d = 0; d < DG; ++d)
+#pragma unroll
+                    for (int q = 0; q < KP; ++q) a[d][q] = v_frag(vl + q * TB, t4, d0 + d);
+                if (use != all) {
+                    if (d0 == 0) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const uint32_t key = 16u * t4 + 8u * (i / 4) + i % 4;
+                            if (!((there >> key) & 1ull)) keep[i / 2] &= i % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+                        }
+                    }
+#pragma unroll
+                    for (int d = 0; d < DG; ++d)
+#pragma unroll
+                        for (int q = 0; q < KP; ++q) a[d][q] &= keep;
                 }
-            }
+                auto mm = [&](int q, const v4u32& w) {
 #pragma unroll
-            for (int d = 0; d < OD; ++d) {
-                v4u32 a[KP];
-#pragma unroll
-                for (int q = 0; q < KP; ++q) a[q] = v_frag(vl + q * TB, t4, d) & keep;
-                auto mm = [&](const v4u32& v, const v4u32& w) {
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(pg_half8, v),
-                                                                  __builtin_bit_cast(pg_half8, w), o[d], 0, 0, 0);
+                    for (int d = 0; d < DG; ++d)
+                        o[d0 + d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(pg_half8, a[d][q]),
+                                                                           __builtin_bit_cast(pg_half8, w), o[d0 + d], 0, 0, 0);
                 };
-                mm(a[0], pp[0][t4]);
-                if constexpr (KP == 2) mm(a[1], pp[0][t4]);
-                mm(a[0], pp[1][t4]);
+                mm(0, pp[0][t4]);
+                if constexpr (KP == 2) mm(1, pp[0][t4]);
+                mm(0, pp[1][t4]);
             }
         }
     }
