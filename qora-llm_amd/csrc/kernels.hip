@@ -1156,12 +1156,12 @@ hipError_t launch_lora_gemm_small(int fmt, const PfSmallParams& q, const LoraPar
     return hipGetLastError();
 }
 
-// Up to 64 rows the waves take the adapters in turn (lora_expand_kernel<true>).
+// Up to 64 rows the waves take a block's adapters in turn (lora_expand_kernel<true>).
 hipError_t launch_lora_expand(const LoraParams& p, const float* part, uint32_t splits, hipStream_t stream) {
     const uint32_t rb = (p.rows + 15u) / 16u;
     if (!lora_ok(p) || rb > 65535u || (splits > 1u && !part)) return hipErrorInvalidValue;
     if (p.rows <= kPfSmallT)
-        hipLaunchKernelGGL((lora_expand_kernel<true>), dim3(p.n / 32u, rb), dim3(256), 0, stream, p, part, splits);
+        hipLaunchKernelGGL((lora_expand_kernel<true>), dim3(p.n / 32u, rb), dim3(512), 0, stream, p, part, splits);
     else
         hipLaunchKernelGGL((lora_expand_kernel<false>), dim3((p.n + 255u) / 256u, rb), dim3(256), 0, stream, p, part, splits);
     return hipGetLastError();

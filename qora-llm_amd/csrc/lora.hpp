@@ -63,27 +63,37 @@ __device__ __forceinline__ f32x4v lr_mma(const v4u32* x, const v4u32* w, f32x4v 
     return c;
 }
 
-// The adapter of row first + lane, -1 without one; lanes from `rows` on have none.
-__device__ __forceinline__ int32_t lr_mine(const LoraParams& p, uint32_t first, uint32_t rows) {
+// The adapter of row first + lane and its entry, e = -1 without one; lanes from `rows` on have none.
+// The entries of all rows come in one load, so that a block's adapters cost it no further trip to memory.
+struct LrMine {
+    int32_t e;
+    LoraEntry a;
+};
+
+__device__ __forceinline__ LrMine lr_mine(const LoraParams& p, uint32_t first, uint32_t rows) {
     const uint32_t lane = threadIdx.x & (kWave - 1), t = first + lane;
-    const int32_t a = p.row_adapter[min(t, p.rows - 1u)];
-    return lane < rows && t < p.rows && a >= 0 && (uint32_t)a < p.count ? a : -1;
+    const int32_t e = p.row_adapter[min(t, p.rows - 1u)];
+    LrMine m;
+    m.e = lane < rows && t < p.rows && e >= 0 && (uint32_t)e < p.count ? e : -1;
+    m.a = p.entries[max(m.e, 0)];
+    return m;
 }
 
-// Takes the next distinct adapter out of `rest` (lanes whose row is still to do).
-__device__ __forceinline__ int32_t lr_next(int32_t mine, uint64_t* rest) {
-    const int32_t e = __builtin_amdgcn_readlane(mine, __builtin_ctzll(*rest));
-    *rest &= ~__ballot(mine == e);
+// The next distinct adapter of `rest` (lanes whose row is still to do), taken out of it; its entry in scalar registers.
+__device__ __forceinline__ int32_t lr_next(const LrMine& m, uint64_t* rest, LoraEntry* a) {
+    const int w = __builtin_ctzll(*rest);
+    const int32_t e = __builtin_amdgcn_readlane(m.e, w);
+    *rest &= ~__ballot(m.e == e);
+    auto word = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, w); };
+    auto ptr = [&](const uint16_t* q) {
+        const uint64_t v = (uint64_t)q;
+        return reinterpret_cast<const uint16_t*>((uint64_t)word((uint32_t)v) | ((uint64_t)word((uint32_t)(v >> 32)) << 32));
+    };
+    a->at = ptr(m.a.at);
+    a->bt = ptr(m.a.bt);
+    a->rp = word(m.a.rp);
+    a->scale = __uint_as_float(word(__float_as_uint(m.a.scale)));
     return e;
-}
-
-__device__ __forceinline__ LoraEntry lr_entry(const LoraParams& p, int32_t e) {
-    LoraEntry a = p.entries[e];
-    a.at = sgpr_ptr(a.at);
-    a.bt = sgpr_ptr(a.bt);
-    a.rp = __builtin_amdgcn_readfirstlane(a.rp);
-    a.scale = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(a.scale)));
-    return a;
 }
 
 constexpr uint32_t kLoraRanks = 32;                          // ranks of a workgroup of the first step
@@ -141,17 +151,17 @@ template <bool VEC>
 __device__ __forceinline__ void lora_shrink_rows(const LoraParams& p, uint32_t slot, uint32_t z, uint32_t rb, float* red) {
     const uint32_t t = threadIdx.x, lane = t & (kWave - 1), g = lane / 16u, li = lane % 16u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(t / kWave);
-    const int32_t mine = lr_mine(p, rb * 16u, 16u);
-    uint64_t rest = __ballot(mine >= 0);
+    const LrMine mine = lr_mine(p, rb * 16u, 16u);
+    uint64_t rest = __ballot(mine.e >= 0);
     const uint32_t kb = z * p.kper, ke = min(p.k, kb + p.kper);
     const float* x = p.x + (uint64_t)min(rb * 16u + li, p.rows - 1u) * p.k;
     const uint32_t chunks = p.rp32 / kLoraRanks, c0 = (slot % chunks) * kLoraRanks;
     slot /= chunks;
     {
         for (uint32_t d = 0; rest; ++d) {
-            const int32_t e = lr_next(mine, &rest);
+            LoraEntry a;
+            const int32_t e = lr_next(mine, &rest, &a);
             if (d % p.slots != slot) continue;
-            const LoraEntry a = lr_entry(p, e);
             if (c0 >= a.rp) continue;
             f32x4v acc[2];
 #pragma unroll
@@ -165,7 +175,7 @@ __device__ __forceinline__ void lora_shrink_rows(const LoraParams& p, uint32_t s
             __syncthreads();
             // (column-major: a lane's four rows are one 16-byte store)
             const uint32_t row = t % 16u;
-            const bool keep = __shfl(mine, (int)row, kWave) == e;
+            const bool keep = __shfl(mine.e, (int)row, kWave) == e;
             float v[2], amax = 0.f;
 #pragma unroll
             for (uint32_t i = 0; i < 2; ++i) {
@@ -229,22 +239,22 @@ struct LoraTile {
 
     __device__ __forceinline__ float add(float v, int i, int r, int c) const { return has[i][r] ? v + sum[i][c][r] : v; }
 
-    __device__ __forceinline__ void get(const LoraParams& p, uint32_t first, int32_t mine, const uint32_t* cols) {
+    __device__ __forceinline__ void get(const LoraParams& p, uint32_t first, const LrMine& mine, const uint32_t* cols) {
         const uint32_t lane = threadIdx.x & (kWave - 1), g = lane / 16u, li = lane % 16u;
         int32_t own[TM];
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-            own[i] = __shfl(mine, (int)(16u * i + li), kWave);
+            own[i] = __shfl(mine.e, (int)(16u * i + li), kWave);
 #pragma unroll
             for (int c = 0; c < CT; ++c) sum[i][c] = f32x4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int r = 0; r < 4; ++r) has[i][r] = __shfl(mine, (int)(16u * i + 4u * g + r), kWave) >= 0;
+            for (int r = 0; r < 4; ++r) has[i][r] = __shfl(mine.e, (int)(16u * i + 4u * g + r), kWave) >= 0;
         }
         const uint32_t nch = p.rp32 / kLoraRanks;
-        uint64_t rest = __ballot(mine >= 0);
+        uint64_t rest = __ballot(mine.e >= 0);
         while (rest) {
-            const int32_t e = lr_next(mine, &rest);
-            const LoraEntry a = lr_entry(p, e);
+            LoraEntry a;
+            const int32_t e = lr_next(mine, &rest, &a);
             for (uint32_t c0 = 0; c0 < a.rp; c0 += 2u * kLoraRanks) {
                 v4u32 bv[2][CT], uh[2][TM], ul[2][TM];
                 int ex[2][TM][4];
@@ -277,7 +287,7 @@ struct LoraTile {
                         for (int x = 0; x < 4; ++x) {
                             uh[s][i][x] &= keep;
                             ul[s][i][x] &= keep;
-                            mine_r[x] = __shfl(mine, (int)(16u * i + 4u * g + x), kWave) == e;
+                            mine_r[x] = __shfl(mine.e, (int)(16u * i + 4u * g + x), kWave) == e;
                         }
 #pragma unroll
                         for (int c = 0; c < CT; ++c) {
@@ -300,17 +310,17 @@ struct LoraTile {
 // the column whose B this lane holds in tile c (past n: any that is not used). The rows' distinct adapters from
 // number d0 on, every step-th.
 template <int CT>
-__device__ __forceinline__ void lora_few_tile(const LoraParams& p, uint32_t first, int32_t mine, const uint32_t* cols,
+__device__ __forceinline__ void lora_few_tile(const LoraParams& p, uint32_t first, const LrMine& mine, const uint32_t* cols,
                                               f32x4v* acc, uint32_t d0, uint32_t step) {
     const uint32_t lane = threadIdx.x & (kWave - 1), g = lane / 16u, li = lane % 16u;
 #pragma unroll
     for (int c = 0; c < CT; ++c) acc[c] = f32x4v{0.f, 0.f, 0.f, 0.f};
-    const int32_t own = __shfl(mine, (int)li, kWave);
-    uint64_t rest = __ballot(mine >= 0);
+    const int32_t own = __shfl(mine.e, (int)li, kWave);
+    uint64_t rest = __ballot(mine.e >= 0);
     for (uint32_t d = 0; rest; ++d) {
-        const int32_t e = lr_next(mine, &rest);
+        LoraEntry a;
+        const int32_t e = lr_next(mine, &rest, &a);
         if (d % step != d0) continue;
-        const LoraEntry a = lr_entry(p, e);
         for (uint32_t r0 = 0; r0 < a.rp; r0 += 32u) {
             const bool in = r0 + 8u * g < a.rp;
             const uint32_t rc = in ? r0 + 8u * g : 0u;
@@ -352,13 +362,12 @@ __device__ __forceinline__ void lora_few_tile(const LoraParams& p, uint32_t firs
 
 // y[t][j] = product + s_e sum_r u[t][r] B_e[r][j], block (columns, row block); the product is y or, with
 // splits > 1, the sum of its K slices in part, in the order of the kernels that sum them without adapters.
-// FEW: 32 columns, the four waves taking the distinct adapters in turn and joining their
-// sums (single tokens: up to 16 adapters a block, so few that the columns have to fill the
-// chip). Else 64 columns a wave.
+// FEW: 32 columns, the eight waves taking the distinct adapters of the block's rows in turn (single tokens: up to
+// 16, which one wave would wait for one after the other). Else 64 columns a wave.
 template <bool FEW>
-__global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p, const float* part, uint32_t splits) {
+__global__ __launch_bounds__(FEW ? 512 : 256) void lora_expand_kernel(LoraParams p, const float* part, uint32_t splits) {
     constexpr int CT = FEW ? 2 : 4;                          // 16-column tiles of a wave
-    __shared__ __align__(16) float red[FEW ? 4 * 16 * 32 : 4];
+    __shared__ __align__(16) float red[FEW ? 8 * 16 * 32 : 4];
     const uint32_t t = threadIdx.x, lane = t & (kWave - 1), g = lane / 16u, li = lane % 16u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(t / kWave);
     const uint32_t rb = blockIdx.y, n0 = FEW ? blockIdx.x * 32u : blockIdx.x * 256u + wave * 64u;
@@ -366,45 +375,46 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p, const fl
     uint32_t cols[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) cols[c] = n0 + 16u * c + li;
-    const int32_t mine = lr_mine(p, rb * 16u, 16u);
+    const LrMine mine = lr_mine(p, rb * 16u, 16u);
     if constexpr (FEW) {
-        // the product's values of this thread's two outputs, on their way while the adapters are
-        const uint32_t row2 = t / 16u, col2 = n0 + 2u * (t % 16u);
-        const uint64_t at2 = (uint64_t)min(rb * 16u + row2, p.rows - 1u) * p.n + min(col2, p.n - 2u);
-        float y0 = 0.f, y1 = 0.f;
-        if (splits > 1u) {
-            for (uint32_t z = 0; z < splits; z += 4u) {
-                float2 q[4];
+        // thread: row t / 32, column t % 32; the product's value on its way while the adapters are
+        const uint32_t row = t / 32u, col = n0 + t % 32u;
+        const bool on = rb * 16u + row < p.rows;
+        const uint64_t at = (uint64_t)min(rb * 16u + row, p.rows - 1u) * p.n + col;   // (n is a multiple of 32)
+        float y = 0.f;
+        if (on) {
+            if (splits > 1u) {
+                for (uint32_t z = 0; z < splits; z += 8u) {
+                    float q[8];
 #pragma unroll
-                for (uint32_t u = 0; u < 4; ++u) q[u] = *reinterpret_cast<const float2*>(part + (uint64_t)min(z + u, splits - 1u) * total + at2);
+                    for (uint32_t u = 0; u < 8; ++u) q[u] = part[(uint64_t)min(z + u, splits - 1u) * total + at];
 #pragma unroll
-                for (uint32_t u = 0; u < 4; ++u)
-                    if (z + u < splits) {
-                        y0 = z + u ? y0 + q[u].x : q[u].x;
-                        y1 = z + u ? y1 + q[u].y : q[u].y;
-                    }
+                    for (uint32_t u = 0; u < 8; ++u)
+                        if (z + u < splits) y = z + u ? y + q[u] : q[u];
+                }
+            } else {
+                y = p.y[at];
             }
-        } else {
-            y0 = p.y[at2];
-            y1 = p.y[at2 + 1];
         }
         f32x4v acc[CT];
-        lora_few_tile<CT>(p, rb * 16u, mine, cols, acc, wave, 4u);
+        lora_few_tile<CT>(p, rb * 16u, mine, cols, acc, wave, 8u);
 #pragma unroll
         for (int c = 0; c < CT; ++c)
             *reinterpret_cast<f32x4v*>(red + wave * 512u + (16u * c + li) * 16u + 4u * g) = acc[c];
         __syncthreads();
-        if (rb * 16u + row2 >= p.rows || col2 >= p.n) return;
-        const uint32_t at = 2u * (t % 16u) * 16u + row2, bt = at + 16u;   // (column-major)
-        const int32_t e = p.row_adapter[rb * 16u + row2];
-        if (e >= 0 && (uint32_t)e < p.count) {
-            // (a row has one adapter: one wave's sum, the others are zero)
-            const float s = p.entries[e].scale;
-            y0 = fmaf(s, (red[at] + red[512u + at]) + (red[1024u + at] + red[1536u + at]), y0);
-            y1 = fmaf(s, (red[bt] + red[512u + bt]) + (red[1024u + bt] + red[1536u + bt]), y1);
+        // the wave of the row's adapter: its number among the distinct ones, by first row, modulo the waves
+        uint64_t rest = __ballot(mine.e >= 0);
+        const int32_t e = __shfl(mine.e, (int)row, kWave);
+        const float s = __shfl(mine.a.scale, (int)row, kWave);
+        uint32_t w = 0, d = 0;
+        while (rest) {
+            LoraEntry a;
+            if (lr_next(mine, &rest, &a) == e) w = d;
+            ++d;
         }
-        p.y[at2] = y0;
-        p.y[at2 + 1] = y1;
+        if (!on) return;
+        if (e >= 0) y = fmaf(s, red[w % 8u * 512u + (t % 32u) * 16u + row], y);   // (column-major)
+        p.y[at] = y;
     } else {
         if (n0 >= p.n) return;
         LoraTile<1, CT> low;
