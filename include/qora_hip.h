@@ -323,7 +323,7 @@ typedef struct {
  * cached positions; position p is slot p % page_size of page
  * pages[s * max_pages + p / page_size]. The three arrays are on the device.
  * Rows from row_start[num_seqs] on belong to nobody and are left as they are.
- * Row offsets ascend from 0 to at most `rows`; offsets that do not, page ids
+ * At most 4096 sequences. Row offsets ascend from 0 to at most `rows`; offsets that do not, page ids
  * outside the pool and lengths past the table reach no memory outside the
  * arrays: what they describe is skipped. */
 typedef struct {
@@ -385,7 +385,7 @@ typedef struct {
  * y[t] = x[t] . W + scale_e (x[t] . A_e) . B_e, e = row_adapter[t] (a device
  * array of `rows` ids); an id outside 0 .. count - 1 means no adapter.
  * lora_upload packs `count` adapters (1 .. 65536) of [k][n] projections once
- * and allocates the workspace of calls of up to max_rows rows; lora_release
+ * and allocates the workspace of calls of up to max_rows rows (1048560 at most); lora_release
  * frees both (refused during capture), and with them ends the use of graphs
  * that recorded a call. The weight's k and n must be the adapters', both
  * multiples of 32. Calls with one lora id use its workspace, and all use

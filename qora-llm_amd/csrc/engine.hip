@@ -2887,7 +2887,7 @@ extern "C" int qora_hip_lora_upload(qora_hip_ctx* c, const qora_lora_adapter* ad
     if (!c) return QORA_HIP_E_INVALID;
     return no_throw([&]() -> int {
         if (!ad || !lora_id) return fail(c, QORA_HIP_E_INVALID, "null argument");
-        if (count == 0 || count > 65536u || max_rows == 0 || max_rows > 0x7FFFFFFFu)
+        if (count == 0 || count > 65536u || max_rows == 0 || max_rows > kLoraMaxRows)
             return fail(c, QORA_HIP_E_INVALID, "bad adapter or row count");
         if (k == 0 || n == 0 || k % 32 != 0 || n % 32 != 0 || k > 0x7FFFFFFFull || n > 0x7FFFFFFFull)
             return fail(c, QORA_HIP_E_INVALID, "adapters need k and n multiples of 32");

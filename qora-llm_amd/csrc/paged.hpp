@@ -195,8 +195,8 @@ __device__ __forceinline__ PagedSeqPlan paged_seq_plan(const PagedAttnParams& p,
     const uint64_t M = (uint64_t)q.n * p.G;
     q.narrow = M <= kPgNarrowRows;
     q.tiles = q.narrow ? (q.n ? 1u : 0u) : (uint32_t)((M + kPgWideRows - 1u) / kPgWideRows);
-    const uint32_t k = q.narrow ? p.narrow_keys : p.wide_keys;
-    q.steps = (q.len + k - 1u) / k;
+    const uint32_t sh = q.narrow ? p.narrow_shift : p.wide_shift;
+    q.steps = (q.len + (1u << sh) - 1u) >> sh;
     return q;
 }
 
@@ -222,11 +222,14 @@ __device__ bool paged_item(const PagedAttnParams& p, uint32_t item, PagedItem* i
         return (float)q.tiles * (float)q.steps * (q.narrow ? p.narrow_cost : p.wide_cost);
     };
     float total = wave_sum(cost_of(q0));
+#pragma unroll 4
     for (uint32_t b = kWave; b < seqs; b += kWave) total += wave_sum(cost_of(paged_seq_plan(p, b + lane)));
     const float share = fmaxf(total * (float)p.g.KVH / p.target, p.least);
     uint64_t base = 0;
+    PagedSeqPlan next = q0;
     for (uint32_t b = 0; b < seqs; b += kWave) {
-        const PagedSeqPlan q = b == 0 ? q0 : paged_seq_plan(p, b + lane);
+        const PagedSeqPlan q = next;
+        if (b + kWave < seqs) next = paged_seq_plan(p, b + kWave + lane);   // (on its way while these are looked through)
         const float per_f = ceilf(share / (q.narrow ? p.narrow_cost : p.wide_cost));
         const uint32_t per = min((uint32_t)fminf(fmaxf(per_f, 1.f), 1e9f), max(q.steps, 1u));
         const uint32_t chunks = max((q.steps + per - 1u) / per, 1u);

@@ -15,7 +15,7 @@
 
 namespace qora {
 
-constexpr uint32_t kPagedMaxSeqs = 65536;
+constexpr uint32_t kPagedMaxSeqs = 4096;
 
 // Position -> slot of its page table entry: false where the position has no
 // place (negative, past the table, or a page id outside the pool).

@@ -442,8 +442,8 @@ struct PagedAttnParams {
     uint32_t H, G;             // query heads, of one KV head
     float scale;               // 1 / sqrt(hd)
     uint32_t page_u, head_u, slot_u;   // the pool's strides in units of 16 bytes
-    // items: keys of a step, its cost, the number of items the work is cut into, the least cost of one
-    uint32_t narrow_keys, wide_keys;
+    // items: keys of a step (log2), its cost, the number of items the work is cut into, the least cost of one
+    uint32_t narrow_shift, wide_shift;
     float narrow_cost, wide_cost, target, least;
     // states of the items of split tiles, and arrivals per tile (zero between launches)
     float* part;

@@ -48,8 +48,8 @@ hipError_t launch_paged_attn(const PagedAttnParams& in, bool f16, int cus, hipSt
     p.head_u = (uint32_t)(p.g.head_stride * es / 16u);
     p.slot_u = (uint32_t)(p.g.slot_stride * es / 16u);
     const bool wide = paged_wide_rows(p.g.max_new, p.G);
-    p.narrow_keys = pg_narrow_keys(f16);
-    p.wide_keys = pg_wide_keys(f16);
+    p.narrow_shift = (uint32_t)__builtin_ctz(pg_narrow_keys(f16));
+    p.wide_shift = (uint32_t)__builtin_ctz(pg_wide_keys(f16));
     // A narrow step (128 binary16 keys of a row or two) takes a workgroup about as long as four wide ones (64 keys of
     // 128 rows): one chunk beside 16 single tokens, calls on one stream / on three, 99.5 / 54.5 us at two, 90.9 / 52.4
     // at four, 98.5 / 52.1 at six. No item is shorter than one narrow step or four wide ones: a state to store

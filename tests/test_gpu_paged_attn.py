@@ -98,6 +98,64 @@ def test_attention_by_the_most_rows(ctx, pkg, kv, max_new):
     assert np.all(np.abs(got[:last] - ref[:last]) <= tol[:last])
 
 
+def test_many_sequences(ctx, pkg):
+    """More sequences than the plan looks at in one go, short and long ones, some with no rows."""
+    r = rng(20)
+    seqs = [(int(r.integers(0, 3)), int(r.integers(1, 40))) for _ in range(1100)]
+    seqs[700] = (1, 2500)
+    seqs[1099] = (20, 300)
+    batch, pool, q = _inputs(pkg, r, "f16", "slot", 8, 4, 2, 64, seqs, pad_rows=1)
+    ref, tol = attention64(pool, batch, q, 4)
+    with device(ctx) as d:
+        got = _run(ctx, pkg, d, pool, batch, q, 4)
+    _check(got, batch, ref, tol)
+
+
+def test_pool_past_32_bits(ctx, pkg):
+    """Pages whose element offsets pass 2^32 and whose bytes pass 2^33: append, then attend, single token and chunk."""
+    r = rng(22)
+    H, KVH, hd, page = 16, 4, 128, 16
+    page_elems = KVH * page * hd
+    num_pages = (9 << 30) // (2 * page_elems)               # 9 GiB of binary16 in each pool
+    assert num_pages * page_elems > 2 ** 32
+    seqs = [(1, 37), (40, 40)]
+    ids = np.array([[num_pages - 1, 3, num_pages - 7], [num_pages - 2, num_pages // 2 + 1, num_pages - 5]], dtype=np.int32)
+    batch = Batch(r, seqs, page)
+    batch.pages, batch.num_pages, batch.max_pages = ids, num_pages, 3
+    dk, dv = ctx.malloc(num_pages * page_elems * 2), ctx.malloc(num_pages * page_elems * 2)
+    try:
+        with device(ctx) as d:
+            kv = pkg.PagedKV(dk, dv, 1, num_pages, page, KVH, hd, page_elems, page * hd, hd)
+            # what the sequences cache, written through the append itself, 37 and 40 rows
+            full = Batch(r, [(37, 37), (40, 40)], page)
+            full.pages, full.num_pages, full.max_pages = ids, num_pages, 3
+            x = r.normal(size=(77, (H + 2 * KVH) * hd)).astype(np.float32)
+            p = d.put(x)
+            ctx.paged_append(kv, full.put(pkg, d), H, p, p + 4 * H * hd, p + 4 * (H + KVH) * hd, x.shape[1], p, q_out_stride=x.shape[1])
+            # a small pool with the same rows, for the definition
+            pool = Pool(pkg, r, "f16", "head", 6, page, KVH, hd, fill=0.0)
+            small = {int(i): n for n, i in enumerate(ids.reshape(-1))}
+            for row, s, pos in full.row_places():
+                at = small[int(ids[s, pos // page])]
+                for h in range(KVH):
+                    pool.k[pool.at(at, h, pos % page)] = x[row].reshape(-1, hd)[H + h]
+                    pool.v[pool.at(at, h, pos % page)] = x[row].reshape(-1, hd)[H + KVH + h]
+            ref_batch = Batch(r, seqs, page)
+            ref_batch.pages = np.vectorize(small.get)(ids).astype(np.int32)
+            ref_batch.num_pages, ref_batch.max_pages = 6, 3
+            q = r.normal(size=(41, H, hd)).astype(np.float32)
+            ref, tol = attention64(pool, ref_batch, q, H)
+            aid = ctx.paged_attn_prepare(41, 2, H, KVH, hd)
+            out = d.put(np.full(q.shape, 77.0, np.float32))
+            ctx.paged_attn_run(aid, kv, batch.put(pkg, d), d.put(q), out)
+            ctx.synchronize()
+            _check(d.get(out, q.shape, np.float32), batch, ref, tol)
+            ctx.paged_attn_release(aid)
+    finally:
+        ctx.free(dk)
+        ctx.free(dv)
+
+
 @pytest.mark.parametrize("kv", ["f16", "f32"])
 def test_rows_that_see_nothing_are_zero(ctx, pkg, kv):
     """Lengths shorter than the new rows, lengths of 0 and below, and pages that are all outside the pool."""
