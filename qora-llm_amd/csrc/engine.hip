@@ -2809,7 +2809,7 @@ extern "C" int qora_hip_paged_attn_prepare(qora_hip_ctx* c, uint32_t max_rows, u
         DeviceGuard dev(c->device);
         HIP_TRY(c, dev.err);
         void* mem;
-        if (int rc = dalloc(c, cb + paged_attn_part_bytes(max_rows, max_seqs, G, num_kv_heads, head_dim, c->cus), &mem))
+        if (int rc = dalloc(c, cb + paged_attn_part_bytes(max_rows, G, head_dim, c->cus), &mem))
             return rc;
         // (waited for: a call on another stream is not ordered behind the context's)
         hipError_t e = hipMemsetAsync(mem, 0, cb, c->stream);
@@ -2920,7 +2920,7 @@ extern "C" int qora_hip_lora_upload(qora_hip_ctx* c, const qora_lora_adapter* ad
         };
         hipError_t e = hipSuccess;
         try {
-            if (int rc = dalloc(c, (uint64_t)kLoraSlices * max_rows * s.rp * sizeof(float), (void**)&s.u)) {
+            if (int rc = dalloc(c, lora_u_bytes(max_rows, s.rp), (void**)&s.u)) {
                 drop();
                 return rc;
             }

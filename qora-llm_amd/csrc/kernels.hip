@@ -1070,6 +1070,12 @@ void lora_shape(LoraParams* p, int cus) {
     p->nz = (p->k + p->kper - 1u) / p->kper;
 }
 
+uint64_t lora_u_bytes(uint64_t rows, uint32_t rp) {
+    const uint64_t few = (uint64_t)kLoraSlices * std::min<uint64_t>(rows, kPfSmallT) * rp * sizeof(float);
+    const uint64_t many = rows * ((uint64_t)rp * 2u * sizeof(uint16_t) + (rp + kLoraRanks - 1u) / kLoraRanks * sizeof(int32_t));
+    return std::max(few, many);
+}
+
 static bool lora_ok(const LoraParams& p) {
     return p.rows > 0 && p.k % 32 == 0 && p.n % 32 == 0 && p.kper % 32 == 0 && p.kper > 0 && p.slots > 0 && p.rp32 >= p.rp && p.rp32 % kLoraRanks == 0 &&
            (uint64_t)p.nz * p.kper >= p.k && (uint64_t)(p.nz - 1u) * p.kper < p.k && (p.rows <= kPfSmallT) == (p.uh == nullptr);

@@ -168,7 +168,7 @@ struct PagedItem {
     uint32_t s, kvh, tile, chunk;
     uint32_t tiles, chunks;
     uint32_t per;              // steps of a chunk
-    uint32_t first;            // item of the tile's chunk 0
+    uint32_t first, state;     // item of the tile's chunk 0, and where its state goes if it is split
     uint32_t row0, n, len;     // the sequence's first row, its rows, keys any of them sees
     int64_t pos0;              // position of its first row
     bool narrow;
@@ -225,7 +225,7 @@ __device__ bool paged_item(const PagedAttnParams& p, uint32_t item, PagedItem* i
 #pragma unroll 4
     for (uint32_t b = kWave; b < seqs; b += kWave) total += wave_sum(cost_of(paged_seq_plan(p, b + lane)));
     const float share = fmaxf(total * (float)p.g.KVH / p.target, p.least);
-    uint64_t base = 0;
+    uint64_t base = 0, split = 0;                             // items before the sequences b .., those of them that are split
     PagedSeqPlan next = q0;
     for (uint32_t b = 0; b < seqs; b += kWave) {
         const PagedSeqPlan q = next;
@@ -235,15 +235,17 @@ __device__ bool paged_item(const PagedAttnParams& p, uint32_t item, PagedItem* i
         const uint32_t chunks = max((q.steps + per - 1u) / per, 1u);
         // (more than any grid has: such a sequence is left out below, and so is what follows it)
         const uint32_t mine = (uint32_t)min((uint64_t)p.g.KVH * q.tiles * chunks, (uint64_t)kPgMaxItems);
-        const uint32_t sum = pg_scan(mine);
+        const uint32_t sum = pg_scan(mine), apart = pg_scan(chunks > 1u ? mine : 0u);
         const uint64_t end = base + sum, begin = end - mine;
         const uint64_t hit = __ballot(item >= begin && item < end);
         if (hit) {
             const int w = __builtin_ctzll(hit);
             auto u = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, w); };
             const uint64_t e0 = base + u(sum), b0 = e0 - u(mine);
-            // row offsets that are none can ask for more items than the grid has: all of such a sequence is left out
-            if (e0 > gridDim.x) return false;
+            // row offsets that are none can ask for more items than the grid has, or states than the workspace: all of
+            // such a sequence is left out
+            const uint64_t s1 = split + u(apart);
+            if (e0 > gridDim.x || (u(chunks) > 1u && s1 > p.states)) return false;
             it->s = b + (uint32_t)w;
             it->tiles = u(q.tiles);
             it->chunks = u(chunks);
@@ -260,9 +262,11 @@ __device__ bool paged_item(const PagedAttnParams& p, uint32_t item, PagedItem* i
             it->tile = r % it->tiles;
             it->chunk = r / it->tiles;
             it->first = (uint32_t)b0 + it->tile * p.g.KVH + it->kvh;
+            it->state = it->chunks > 1u ? (uint32_t)(s1 - u(mine)) + it->tile * p.g.KVH + it->kvh : 0u;
             return true;
         }
         base += (uint32_t)__builtin_amdgcn_readlane((int)sum, kWave - 1);
+        split += (uint32_t)__builtin_amdgcn_readlane((int)apart, kWave - 1);
         if (base > item) return false;
     }
     return false;
@@ -714,7 +718,7 @@ __device__ __forceinline__ void paged_narrow(const PagedAttnParams& p, const Pag
     }
     if (it.chunks > 1u) {
         const uint32_t stride = it.tiles * g.KVH;            // items of a tile's neighbouring chunks
-        auto state = [&](uint32_t c) { return p.part + (uint64_t)(it.first + c * stride) * p.part_floats; };
+        auto state = [&](uint32_t c) { return p.part + (uint64_t)(it.state + c * stride) * p.part_floats; };
         if (row < M) {
             float* d = state(it.chunk);
 #pragma unroll
@@ -1204,7 +1208,7 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
         // states in lane order: piece (wave, j) of 64 lanes x 16 bytes, then m, l a lane
         constexpr uint32_t NJ = HD / 8;
         const uint32_t stride = it.tiles * g.KVH;
-        auto state = [&](uint32_t c) { return p.part + (uint64_t)(it.first + c * stride) * p.part_floats; };
+        auto state = [&](uint32_t c) { return p.part + (uint64_t)(it.state + c * stride) * p.part_floats; };
         if (wave_on) {
             float* b = state(it.chunk);
 #pragma unroll

@@ -445,9 +445,9 @@ struct PagedAttnParams {
     // items: keys of a step (log2), its cost, the number of items the work is cut into, the least cost of one
     uint32_t narrow_shift, wide_shift;
     float narrow_cost, wide_cost, target, least;
-    // states of the items of split tiles, and arrivals per tile (zero between launches)
+    // states of the items of split tiles (as many as there can be), and arrivals per tile (zero between launches)
     float* part;
-    uint32_t part_floats;
+    uint32_t part_floats, states;
     uint32_t* count;
 };
 

@@ -35,9 +35,12 @@ uint64_t paged_attn_items(uint64_t rows, uint64_t seqs, uint32_t G, uint32_t KVH
 
 static bool paged_wide_rows(uint64_t max_new, uint32_t G) { return max_new * G > kPgNarrowRows; }
 
-uint64_t paged_attn_part_bytes(uint64_t rows, uint64_t seqs, uint32_t G, uint32_t KVH, uint32_t hd, int cus) {
-    return paged_attn_items(rows, seqs, G, KVH, cus) * pg_part_floats(hd <= 64 ? 64 : 128, paged_wide_rows(rows, G)) *
-           sizeof(float);
+// Items of split tiles: a tile is split when it has more than an item's share of the work, so there are at most
+// `target` such tiles, and their items are at most that share's count and one more each.
+static uint32_t paged_states(int cus) { return 2u * paged_target(cus) + 2u; }
+
+uint64_t paged_attn_part_bytes(uint64_t rows, uint32_t G, uint32_t hd, int cus) {
+    return (uint64_t)paged_states(cus) * pg_part_floats(hd <= 64 ? 64 : 128, paged_wide_rows(rows, G)) * sizeof(float);
 }
 
 hipError_t launch_paged_attn(const PagedAttnParams& in, bool f16, int cus, hipStream_t stream) {
@@ -59,6 +62,7 @@ hipError_t launch_paged_attn(const PagedAttnParams& in, bool f16, int cus, hipSt
     p.target = (float)paged_target(cus);
     p.least = 4.f;
     p.part_floats = pg_part_floats(HD, wide);
+    p.states = paged_states(cus);
     const uint64_t items = paged_attn_items(p.g.rows, p.g.seqs, p.G, p.g.KVH, cus);
     if (items > kPgMaxItems) return hipErrorInvalidValue;
     const dim3 grid((uint32_t)items), block(256);
