@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from helpers import device, rng
-from paged_util import Batch, Pool, attention64
+from paged_util import EPS32, Batch, Pool, attention64
 
 pytestmark = pytest.mark.gpu
 
@@ -108,6 +108,34 @@ def test_many_sequences(ctx, pkg):
     ref, tol = attention64(pool, batch, q, 4)
     with device(ctx) as d:
         got = _run(ctx, pkg, d, pool, batch, q, 4)
+    _check(got, batch, ref, tol)
+
+
+@pytest.mark.parametrize("rows,keys", [(1, 43 * 128), (20, 43 * 64)])
+def test_every_tile_split(ctx, pkg, rows, keys):
+    """As many split tiles as there can be: equal sequences, a few fewer than the work is cut into (two items for
+    each of 256 CUs), so that each has a little more than an item's share; they read the same pages."""
+    r = rng(24)
+    page, n = 256, 500
+    batch = Batch(r, [(rows, keys)] * n, page)
+    batch.num_pages = batch.max_pages = -(-keys // page)
+    batch.pages = np.tile(r.permutation(batch.num_pages).astype(np.int32), (n, 1))
+    pool = Pool(pkg, r, "f16", "head", batch.num_pages, page, 1, 64, fill=0.0)
+    k, v = np.zeros((2, keys, 64))
+    for j in range(keys):
+        p, slot = batch.place(0, j)
+        for x, plain in ((pool.k, k), (pool.v, v)):
+            x[pool.at(p, 0, slot)] = r.normal(size=64).astype(np.float16)
+            plain[j] = x[pool.at(p, 0, slot)]
+    q = r.normal(size=(batch.rows, 1, 64)).astype(np.float32)
+    sc = (q[:, 0].astype(np.float64) @ k.T / 8).reshape(n, rows, keys)
+    sc[:, np.arange(keys) > keys - rows + np.arange(rows)[:, None]] = -np.inf
+    e = np.exp(sc - sc.max(-1, keepdims=True))
+    ref = (e @ v / e.sum(-1, keepdims=True)).reshape(-1, 1, 64)
+    S = (np.abs(q[:, 0]).astype(np.float64) @ np.abs(k).T / 8).max(-1)
+    tol = EPS32 * (2 * (64 + 16) * S + keys + 64)[:, None, None] * np.abs(v).max()
+    with device(ctx) as d:
+        got = _run(ctx, pkg, d, pool, batch, q, 1)
     _check(got, batch, ref, tol)
 
 
