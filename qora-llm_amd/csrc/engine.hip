@@ -2267,8 +2267,8 @@ uint64_t pf_gemm_reserve(int fmt, uint32_t T, uint32_t K, uint32_t N, int cus) {
 
 namespace {
 
-// qora_hip_gemm; with `lora` (its shape set), the adapters' two steps around the product.
-int gemm_call(qora_hip_ctx* c, uint32_t wid, const float* x, float* y, uint64_t rows, void* stream, const LoraParams* lora) {
+// qora_hip_gemm; with `lora`, the adapters' two steps around the product.
+int gemm_call(qora_hip_ctx* c, uint32_t wid, const float* x, float* y, uint64_t rows, void* stream, LoraParams* lora) {
     if (!x || !y) return fail(c, QORA_HIP_E_INVALID, "null argument");
     if (!get_weight(c, wid)) return fail(c, QORA_HIP_E_INVALID, "unknown weight id");
     DevWeight* w = &c->weights[wid];
@@ -2302,6 +2302,7 @@ int gemm_call(qora_hip_ctx* c, uint32_t wid, const float* x, float* y, uint64_t 
     }
     if (int rc = ensure_pf_ws(c, need)) return rc;
     c->ws_pf_captured = c->ws_pf_captured || captured(c, s);
+    if (lora) lora_shape(lora, !small && g.wide && g.s2.splits <= 1u, c->cus);
     if (small) {
         PfSmallParams q{};
         q.x = x;
@@ -2331,12 +2332,12 @@ int gemm_call(qora_hip_ctx* c, uint32_t wid, const float* x, float* y, uint64_t 
     r.xh = (uint16_t*)base;
     r.xl = (uint16_t*)(base + g.bx);
     r.xe = (int32_t*)(base + 2 * g.bx);
-    // (x . A in or ahead of the launch that prepares the product, which may write y over x)
+    // (x . A in the launch that prepares the product, which may write y over x)
+    if (lora)
+        HIP_TRY(c, launch_lora_gemm_prep(*lora, r.xh, r.xl, r.xe, g.wide && q4 ? (const uint8_t*)w->w : nullptr,
+                                         (const uint16_t*)w->scales, (uint2*)wq, (uint16_t*)(wq + g.bq), s));
     if (g.wide) {
-        if (lora && !q4) HIP_TRY(c, launch_lora_shrink(*lora, s));
-        if (lora && q4)
-            HIP_TRY(c, launch_lora_gemm_prep(*lora, r.xh, r.xl, r.xe, (const uint8_t*)w->w, (const uint16_t*)w->scales,
-                                             (uint2*)wq, (uint16_t*)(wq + g.bq), s));
+        if (lora) {}
         else if (q4) HIP_TRY(c, launch_pf_gemm_prep(x, T, r.xh, r.xl, r.xe, (const uint8_t*)w->w, (const uint16_t*)w->scales,
                                                K, N, (uint2*)wq, (uint16_t*)(wq + g.bq), s));
         else HIP_TRY(c, launch_pf_rows(PF_ROW_SPLIT, r, T, s));
@@ -2356,8 +2357,7 @@ int gemm_call(qora_hip_ctx* c, uint32_t wid, const float* x, float* y, uint64_t 
         else HIP_TRY(c, launch_pf_gemm2(g.s2.bm, h, s, true, q4 ? PF_W_RAW : PF_W_F16));
         return QORA_HIP_OK;
     }
-    if (lora) HIP_TRY(c, launch_lora_shrink(*lora, s));
-    HIP_TRY(c, launch_pf_rows(PF_ROW_SPLIT, r, T, s));
+    if (!lora) HIP_TRY(c, launch_pf_rows(PF_ROW_SPLIT, r, T, s));
     int8_t* wf = (int8_t*)(base + 2 * g.bx + g.be);
     if (q4)
         HIP_TRY(c, launch_pf_weight_exp((const uint16_t*)w->scales, K, N / 32, wf, (uint32_t*)(base + 2 * g.bx + g.be + g.bf), s));
@@ -2920,7 +2920,7 @@ extern "C" int qora_hip_lora_upload(qora_hip_ctx* c, const qora_lora_adapter* ad
         };
         hipError_t e = hipSuccess;
         try {
-            if (int rc = dalloc(c, lora_u_bytes(max_rows, s.rp), (void**)&s.u)) {
+            if (int rc = dalloc(c, lora_u_bytes(max_rows, s.rp, c->cus), (void**)&s.u)) {
                 drop();
                 return rc;
             }
@@ -3000,7 +3000,6 @@ extern "C" int qora_hip_gemm_lora(qora_hip_ctx* c, uint32_t wid, uint32_t lora_i
         p.x = x;
         p.y = y;
         p.u = s.u;
-        lora_shape(&p, c->cus);
         return gemm_call(c, wid, x, y, rows, stream, &p);
     });
 }

@@ -1053,41 +1053,50 @@ hipError_t launch_pf_attn(const PrefillAttnParams& p, hipStream_t stream) {
 
 // ---- low-rank adapters ----
 
-// K slices of the adapters' first step, of few tokens: enough workgroups for two a CU, of at
-// least 512 rows (four waves of 128), and at most eight, which the second step adds up.
-void lora_shape(LoraParams* p, int cus) {
+// Workgroups of a row block that share its distinct adapters: one for each where there are few blocks (their rows are
+// often single tokens'), four for more, whose rows are prompts' and have one adapter or two a block.
+static uint32_t lora_slot_count(uint64_t rb) { return rb <= 16u ? 16u : 4u; }
+
+// K slices of the adapters' first step, for the second to add up: enough workgroups for two a CU, and at most eight.
+static uint32_t lora_slices(uint64_t rb, int cus) {
+    const uint64_t per = rb * lora_slot_count(rb), want = (2u * (uint64_t)std::max(1, cus) + per - 1u) / per;
+    return (uint32_t)std::max<uint64_t>(1u, std::min<uint64_t>(want, kLoraSlices));
+}
+
+// Slices are of at least 512 rows of K (four waves of 128). The product's kernel takes the sums of one, ready to
+// multiply, in u's memory: slices joined ahead of it by the last to arrive won nothing beside the packing of the
+// weight (65 .. 1024 rows, 2048 and 8192 rows of K) and cost 3 us at 512 rows of rank 64.
+void lora_shape(LoraParams* p, bool in_product, int cus) {
     const uint32_t rb = (p->rows + 15u) / 16u;
-    p->slots = rb <= 4u ? 16u : 4u;
+    p->slots = lora_slot_count(rb);
     p->rp32 = (p->rp + kLoraRanks - 1u) / kLoraRanks * kLoraRanks;
-    const uint32_t want = (2u * (uint32_t)std::max(1, cus) + rb * p->slots - 1u) / (rb * p->slots);
-    // (a prompt's rows: one, whose sums go out ready to multiply, in the same memory)
-    const bool few = p->rows <= kPfSmallT;
-    const uint32_t nz = few ? std::max(1u, std::min({want, (p->k + 511u) / 512u, kLoraSlices})) : 1u;
-    p->uh = few ? nullptr : reinterpret_cast<uint16_t*>(p->u);
-    p->ul = few ? nullptr : p->uh + (uint64_t)p->rows * p->rp;
-    p->ue = few ? nullptr : reinterpret_cast<int32_t*>(p->ul + (uint64_t)p->rows * p->rp);
+    const uint32_t nz = in_product ? 1u : std::max(1u, std::min(lora_slices(rb, cus), (p->k + 511u) / 512u));
+    p->uh = in_product ? reinterpret_cast<uint16_t*>(p->u) : nullptr;
+    p->ul = in_product ? p->uh + (uint64_t)p->rows * p->rp : nullptr;
+    p->ue = in_product ? reinterpret_cast<int32_t*>(p->ul + (uint64_t)p->rows * p->rp) : nullptr;
     p->kper = ((p->k + nz - 1u) / nz + 31u) / 32u * 32u;
     p->nz = (p->k + p->kper - 1u) / p->kper;
 }
 
-uint64_t lora_u_bytes(uint64_t rows, uint32_t rp) {
-    const uint64_t few = (uint64_t)kLoraSlices * std::min<uint64_t>(rows, kPfSmallT) * rp * sizeof(float);
-    const uint64_t many = rows * ((uint64_t)rp * 2u * sizeof(uint16_t) + (rp + kLoraRanks - 1u) / kLoraRanks * sizeof(int32_t));
-    return std::max(few, many);
+uint64_t lora_u_bytes(uint64_t rows, uint32_t rp, int cus) {
+    // (of one slice: the two parts and the exponents)
+    uint64_t b = rows * ((uint64_t)rp + (rp + kLoraRanks - 1u) / kLoraRanks) * sizeof(float);
+    for (uint64_t rb = 1; rb <= (rows + 15u) / 16u; ++rb) {
+        const uint64_t nz = lora_slices(rb, cus);
+        if (nz == 1u && rb > 16u) break;                     // (and so are all beyond)
+        b = std::max(b, nz * std::min(rows, 16u * rb) * rp * sizeof(float));
+    }
+    return b;
 }
 
 static bool lora_ok(const LoraParams& p) {
-    return p.rows > 0 && p.k % 32 == 0 && p.n % 32 == 0 && p.kper % 32 == 0 && p.kper > 0 && p.slots > 0 && p.rp32 >= p.rp && p.rp32 % kLoraRanks == 0 &&
-           (uint64_t)p.nz * p.kper >= p.k && (uint64_t)(p.nz - 1u) * p.kper < p.k && (p.rows <= kPfSmallT) == (p.uh == nullptr);
+    return p.rows > 0 && p.k % 32 == 0 && p.n % 32 == 0 && p.kper % 32 == 0 && p.kper > 0 && p.slots > 0 && p.rp32 >= p.rp &&
+           p.rp32 % kLoraRanks == 0 && (uint64_t)p.nz * p.kper >= p.k && (uint64_t)(p.nz - 1u) * p.kper < p.k &&
+           p.nz <= kLoraSlices && (!p.uh || p.nz == 1u);
 }
 
-__global__ __launch_bounds__(256) void lora_shrink_kernel(LoraParams p) {
-    __shared__ __align__(16) float red[kLoraShrinkLds / 4];
-    lora_shrink_block(p, blockIdx.x, blockIdx.y, blockIdx.z, red);
-}
-
-// The product's operand split and weight packing (pf_gemm_prep_kernel) and the adapters' first step in
-// one launch: both read x, and each leaves much of the chip idle by itself.
+// The product's operand split and weight packing (pf_gemm_prep_kernel; w null: no packing) and the adapters' first
+// step in one launch: both read x, and each leaves much of the chip idle by itself.
 __global__ __launch_bounds__(256, 4) void lora_gemm_prep_kernel(LoraParams p, uint32_t nshrink, uint16_t* xh, uint16_t* xl,
                                                                 int32_t* xe, const uint8_t* w, const uint16_t* scales,
                                                                 uint2* wq, uint16_t* sc) {
@@ -1109,9 +1118,9 @@ __global__ __launch_bounds__(256, BM == 64 && WM == PF_W_F16 ? 2 : 4) void lora_
 
 hipError_t launch_lora_gemm_prep(const LoraParams& p, uint16_t* xh, uint16_t* xl, int32_t* xe, const uint8_t* w,
                                  const uint16_t* scales, uint2* wq, uint16_t* sc, hipStream_t stream) {
-    if (!lora_ok(p) || !pf_gemm2_supported(p.k, p.n)) return hipErrorInvalidValue;
+    if (!lora_ok(p) || (w && !pf_gemm2_supported(p.k, p.n))) return hipErrorInvalidValue;
     const uint64_t ns = (uint64_t)lora_slots(p) * p.nz * ((p.rows + 15u) / 16u);
-    const uint64_t grid = ns + p.rows + (uint64_t)(p.n / 128u) * ((p.k / 32u + 1u) / 2u);
+    const uint64_t grid = ns + p.rows + (w ? (uint64_t)(p.n / 128u) * ((p.k / 32u + 1u) / 2u) : 0u);
     if (grid > 0x7FFFFFFFull) return hipErrorInvalidValue;
     hipLaunchKernelGGL(lora_gemm_prep_kernel, dim3((uint32_t)grid), dim3(256), 0, stream, p, (uint32_t)ns, xh, xl, xe, w,
                        scales, wq, sc);
@@ -1123,7 +1132,7 @@ hipError_t launch_lora_gemm2(uint32_t bm, const PfGemm2Params& q, const LoraPara
         if (const hipError_t e = launch_pf_gemm2(bm, q, stream, false, wm)) return e;
         return launch_lora_expand(p, q.part, q.splits, stream);
     }
-    if (!lora_ok(p) || !pf_gemm2_ok(bm, q, wm) || q.nseg != 1 || q.swiglu || q.T != p.rows || q.k != p.k || q.ntot != p.n ||
+    if (!lora_ok(p) || !p.uh || !pf_gemm2_ok(bm, q, wm) || q.nseg != 1 || q.swiglu || q.T != p.rows || q.k != p.k || q.ntot != p.n ||
         wm == PF_W_PACKED || q.seg[0].accumulate)
         return hipErrorInvalidValue;
     const dim3 grid(q.ntot / 128u, (q.T + bm - 1) / bm);
@@ -1135,13 +1144,6 @@ hipError_t launch_lora_gemm2(uint32_t bm, const PfGemm2Params& q, const LoraPara
     if (wm == PF_W_RAW) QORA_LORA_GEMM2(PF_W_RAW);
     else QORA_LORA_GEMM2(PF_W_F16);
 #undef QORA_LORA_GEMM2
-    return hipGetLastError();
-}
-
-hipError_t launch_lora_shrink(const LoraParams& p, hipStream_t stream) {
-    const uint32_t rb = (p.rows + 15u) / 16u;
-    if (!lora_ok(p) || rb > 65535u) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(lora_shrink_kernel, dim3(lora_slots(p), p.nz, rb), dim3(256), 0, stream, p);
     return hipGetLastError();
 }
 
@@ -1162,14 +1164,15 @@ hipError_t launch_lora_gemm_small(int fmt, const PfSmallParams& q, const LoraPar
     return hipGetLastError();
 }
 
-// Up to 64 rows the waves take a block's adapters in turn (lora_expand_kernel<true>).
+// 32 columns a workgroup, all its waves on them, or 128 with two waves a 32 where those are many (512 rows of
+// one adapter or two a block, 11008 columns, binary16: 133 us against 110).
 hipError_t launch_lora_expand(const LoraParams& p, const float* part, uint32_t splits, hipStream_t stream) {
     const uint32_t rb = (p.rows + 15u) / 16u;
-    if (!lora_ok(p) || rb > 65535u || (splits > 1u && !part)) return hipErrorInvalidValue;
-    if (p.rows <= kPfSmallT)
-        hipLaunchKernelGGL((lora_expand_kernel<true>), dim3(p.n / 32u, rb), dim3(512), 0, stream, p, part, splits);
+    if (!lora_ok(p) || p.uh || rb > 65535u || (splits > 1u && !part)) return hipErrorInvalidValue;
+    if ((uint64_t)rb * (p.n / 32u) >= 2048u)
+        hipLaunchKernelGGL((lora_expand_kernel<4>), dim3((p.n + 127u) / 128u, rb), dim3(512), 0, stream, p, part, splits);
     else
-        hipLaunchKernelGGL((lora_expand_kernel<false>), dim3((p.n + 255u) / 256u, rb), dim3(256), 0, stream, p, part, splits);
+        hipLaunchKernelGGL((lora_expand_kernel<1>), dim3(p.n / 32u, rb), dim3(512), 0, stream, p, part, splits);
     return hipGetLastError();
 }
 

@@ -182,11 +182,10 @@ uint64_t paged_attn_items(uint64_t rows, uint64_t seqs, uint32_t G, uint32_t KVH
 uint64_t paged_attn_part_bytes(uint64_t rows, uint32_t G, uint32_t hd, int cus);
 // p.part and p.count hold that; part_floats, states, the strides in units and the item costs are set here.
 hipError_t launch_paged_attn(const PagedAttnParams& p, bool f16, int cus, hipStream_t stream);
-constexpr uint32_t kLoraSlices = 8;   // K slices of x . A at most
 constexpr uint32_t kLoraMaxRows = 16u * 65535u;   // a grid dimension of row blocks
-uint64_t lora_u_bytes(uint64_t rows, uint32_t rp);   // u of calls of up to that many rows
-void lora_shape(LoraParams* p, int cus);   // sets nz, kper, slots and u's form for p's k, rows and u
-hipError_t launch_lora_shrink(const LoraParams& p, hipStream_t stream);
+uint64_t lora_u_bytes(uint64_t rows, uint32_t rp, int cus);   // u of calls of up to that many rows
+// Sets nz, kper, slots and u's form (in_product: for launch_lora_gemm2 of one slice) for p's k, rows and u.
+void lora_shape(LoraParams* p, bool in_product, int cus);
 // launch_lora_shrink and the product kernel of launch_pf_gemm_small in one launch, without the sum over
 // q.splits slices: launch_lora_expand takes q.part and q.splits and adds them up itself (splits 1: it adds to y)
 hipError_t launch_lora_gemm_small(int fmt, const PfSmallParams& q, const LoraParams& p, hipStream_t stream);

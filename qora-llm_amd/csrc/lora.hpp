@@ -96,6 +96,7 @@ __device__ __forceinline__ int32_t lr_next(const LrMine& m, uint64_t* rest, Lora
     return e;
 }
 
+constexpr uint32_t kLoraSlices = 8;                          // K slices of x . A at most
 constexpr uint32_t kLoraRanks = 32;                          // ranks of a workgroup of the first step
 constexpr uint32_t kLoraShrinkLds = 4u * 16u * kLoraRanks * 4u;
 
@@ -360,82 +361,76 @@ __device__ __forceinline__ void lora_few_tile(const LoraParams& p, uint32_t firs
     }
 }
 
-// y[t][j] = product + s_e sum_r u[t][r] B_e[r][j], block (columns, row block); the product is y or, with
+// y[t][j] = product + s_e sum_r u[t][r] B_e[r][j], block (32 CG columns, 16 rows); the product is y or, with
 // splits > 1, the sum of its K slices in part, in the order of the kernels that sum them without adapters.
-// FEW: 32 columns, the eight waves taking the distinct adapters of the block's rows in turn (single tokens: up to
-// 16, which one wave would wait for one after the other). Else 64 columns a wave.
-template <bool FEW>
-__global__ __launch_bounds__(FEW ? 512 : 256) void lora_expand_kernel(LoraParams p, const float* part, uint32_t splits) {
-    constexpr int CT = FEW ? 2 : 4;                          // 16-column tiles of a wave
-    __shared__ __align__(16) float red[FEW ? 8 * 16 * 32 : 4];
+// The 8 / CG waves of 32 columns take the distinct adapters of the block's rows in turn (single tokens: up to
+// 16, which one wave would wait for one after the other).
+template <int CG>
+__global__ __launch_bounds__(512) void lora_expand_kernel(LoraParams p, const float* part, uint32_t splits) {
+    constexpr int CT = 2;                                    // 16-column tiles of a wave
+    constexpr uint32_t W = 8u / CG;
+    __shared__ __align__(16) float red[8 * 16 * 32];
     const uint32_t t = threadIdx.x, lane = t & (kWave - 1), g = lane / 16u, li = lane % 16u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(t / kWave);
-    const uint32_t rb = blockIdx.y, n0 = FEW ? blockIdx.x * 32u : blockIdx.x * 256u + wave * 64u;
+    const uint32_t rb = blockIdx.y, n0 = blockIdx.x * 32u * CG;
     const uint64_t total = (uint64_t)p.rows * p.n;
     uint32_t cols[CT];
 #pragma unroll
-    for (int c = 0; c < CT; ++c) cols[c] = n0 + 16u * c + li;
+    for (int c = 0; c < CT; ++c) cols[c] = n0 + wave / W * 32u + 16u * c + li;
     const LrMine mine = lr_mine(p, rb * 16u, 16u);
-    if constexpr (FEW) {
-        // thread: row t / 32, column t % 32; the product's value on its way while the adapters are
-        const uint32_t row = t / 32u, col = n0 + t % 32u;
-        const bool on = rb * 16u + row < p.rows;
-        const uint64_t at = (uint64_t)min(rb * 16u + row, p.rows - 1u) * p.n + col;   // (n is a multiple of 32)
-        float y = 0.f;
-        if (on) {
-            if (splits > 1u) {
-                for (uint32_t z = 0; z < splits; z += 8u) {
-                    float q[8];
+    // thread: row t / 32, columns t % 32 and 32 further; the product's values on their way while the adapters are
+    const uint32_t row = t / 32u;
+    const bool on = rb * 16u + row < p.rows;
+    const uint64_t at = (uint64_t)min(rb * 16u + row, p.rows - 1u) * p.n;
+    uint64_t to[CG];
+    float y[CG];
 #pragma unroll
-                    for (uint32_t u = 0; u < 8; ++u) q[u] = part[(uint64_t)min(z + u, splits - 1u) * total + at];
+    for (int j = 0; j < CG; ++j) {
+        to[j] = at + min(n0 + 32u * j + t % 32u, p.n - 1u);  // (n is a multiple of 32)
+        y[j] = 0.f;
+    }
+    if (on) {
+        if (splits > 1u) {
+            constexpr uint32_t Z = 8u / CG;
+            for (uint32_t z = 0; z < splits; z += Z) {
+                float q[CG][Z];
 #pragma unroll
-                    for (uint32_t u = 0; u < 8; ++u)
-                        if (z + u < splits) y = z + u ? y + q[u] : q[u];
-                }
-            } else {
-                y = p.y[at];
+                for (uint32_t u = 0; u < Z; ++u)
+#pragma unroll
+                    for (int j = 0; j < CG; ++j) q[j][u] = part[(uint64_t)min(z + u, splits - 1u) * total + to[j]];
+#pragma unroll
+                for (uint32_t u = 0; u < Z; ++u)
+#pragma unroll
+                    for (int j = 0; j < CG; ++j)
+                        if (z + u < splits) y[j] = z + u ? y[j] + q[j][u] : q[j][u];
             }
-        }
-        f32x4v acc[CT];
-        lora_few_tile<CT>(p, rb * 16u, mine, cols, acc, wave, 8u);
+        } else {
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
-            *reinterpret_cast<f32x4v*>(red + wave * 512u + (16u * c + li) * 16u + 4u * g) = acc[c];
-        __syncthreads();
-        // the wave of the row's adapter: its number among the distinct ones, by first row, modulo the waves
-        uint64_t rest = __ballot(mine.e >= 0);
-        const int32_t e = __shfl(mine.e, (int)row, kWave);
-        const float s = __shfl(mine.a.scale, (int)row, kWave);
-        uint32_t w = 0, d = 0;
-        while (rest) {
-            LoraEntry a;
-            if (lr_next(mine, &rest, &a) == e) w = d;
-            ++d;
+            for (int j = 0; j < CG; ++j) y[j] = p.y[to[j]];
         }
-        if (!on) return;
-        if (e >= 0) y = fmaf(s, red[w % 8u * 512u + (t % 32u) * 16u + row], y);   // (column-major)
-        p.y[at] = y;
-    } else {
-        if (n0 >= p.n) return;
-        LoraTile<1, CT> low;
-        low.get(p, rb * 16u, mine, cols);
+    }
+    f32x4v acc[CT];
+    lora_few_tile<CT>(p, rb * 16u, mine, cols, acc, wave % W, W);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const uint32_t row = rb * 16u + 4u * g + r;
+    for (int c = 0; c < CT; ++c)
+        *reinterpret_cast<f32x4v*>(red + wave * 512u + (16u * c + li) * 16u + 4u * g) = acc[c];
+    __syncthreads();
+    // the wave of the row's adapter: its number among the distinct ones, by first row, modulo the waves
+    uint64_t rest = __ballot(mine.e >= 0);
+    const int32_t e = __shfl(mine.e, (int)row, kWave);
+    const float s = __shfl(mine.a.scale, (int)row, kWave);
+    uint32_t w = 0, d = 0;
+    while (rest) {
+        LoraEntry a;
+        if (lr_next(mine, &rest, &a) == e) w = d;
+        ++d;
+    }
+    if (!on) return;
 #pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                if (row >= p.rows || cols[c] >= p.n || (splits <= 1u && !low.has[0][r])) continue;
-                const uint64_t at = (uint64_t)row * p.n + cols[c];
-                float v;
-                if (splits > 1u) {
-                    v = part[at];
-                    for (uint32_t z = 1; z < splits; ++z) v += part[(uint64_t)z * total + at];
-                } else {
-                    v = p.y[at];
-                }
-                p.y[at] = low.add(v, 0, r, c);
-            }
-        }
+    for (int j = 0; j < CG; ++j) {
+        if (n0 + 32u * j >= p.n) break;
+        if (e >= 0) y[j] = fmaf(s, red[(j * W + w % W) * 512u + (t % 32u) * 16u + row], y[j]);   // (column-major)
+        p.y[to[j]] = y[j];
     }
 }
 

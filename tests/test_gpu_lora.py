@@ -62,6 +62,12 @@ CASES = [
     ("q4", 11008, 2048, [64, 16], 5, 2),
     ("q4", 1056, 1088, [16, 32, 100], 17, 17),
     ("q4", 2048, 11008, [64] * 4, 130, 40),
+    ("q4", 2048, 512, [16] * 20, 65, 1),               # many tokens, several K slices of x A
+    ("f16", 4096, 256, [64, 16, 100], 96, 2),
+    ("q4", 5024, 256, [33, 1, 256], 257, 40),
+    ("f16", 2080, 160, [17, 40, 8], 1100, 300),
+    ("f16", 608, 2080, [5, 48] * 9, 1031, 3),          # many columns and rows, many adapters a block
+    ("q4", 1024, 4224, [32] * 5, 400, 2),
 ]
 
 
