@@ -2377,8 +2377,8 @@ int gemm_call(qora_hip_ctx* c, uint32_t wid, const float* x, float* y, uint64_t 
     h.splits = g.sh.splits;
     h.kper = g.sh.kper;
     h.part = part;
-    HIP_TRY(c, launch_pf_gemm(w->fmt, h, s));
-    if (lora) HIP_TRY(c, launch_lora_expand(*lora, nullptr, 1, s));
+    HIP_TRY(c, launch_pf_gemm(w->fmt, h, s, !lora));
+    if (lora) HIP_TRY(c, launch_lora_expand(*lora, part, h.splits, s));
     return QORA_HIP_OK;
 }
 

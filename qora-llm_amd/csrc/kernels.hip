@@ -741,7 +741,7 @@ PfGemmShape pf_gemm_shape(uint32_t T, uint32_t k, uint32_t n, int cus) {
     return sh;
 }
 
-hipError_t launch_pf_gemm(int fmt, const PrefillGemmParams& p, hipStream_t stream) {
+hipError_t launch_pf_gemm(int fmt, const PrefillGemmParams& p, hipStream_t stream, bool reduce) {
     if (!pf_gemm_supported(p.k, p.n) || p.T == 0 || p.splits == 0 || p.kper % 32 != 0 ||
         (uint64_t)p.splits * p.kper < p.k || (p.splits > 1 && !p.part))
         return hipErrorInvalidValue;
@@ -763,7 +763,7 @@ hipError_t launch_pf_gemm(int fmt, const PrefillGemmParams& p, hipStream_t strea
         else QORA_PF_GEMM(64, false);
     }
 #undef QORA_PF_GEMM
-    if (p.splits > 1) {
+    if (p.splits > 1 && reduce) {
         const uint64_t total = (uint64_t)p.T * p.n;
         const uint32_t blocks = (uint32_t)std::min<uint64_t>(4096, (total + 255) / 256);
         hipLaunchKernelGGL(pf_splitk_reduce_kernel, dim3(blocks), dim3(256), 0, stream, p);
@@ -1053,13 +1053,10 @@ hipError_t launch_pf_attn(const PrefillAttnParams& p, hipStream_t stream) {
 
 // ---- low-rank adapters ----
 
-// Workgroups of a row block that share its distinct adapters: one for each where there are few blocks (their rows are
-// often single tokens'), four for more, whose rows are prompts' and have one adapter or two a block.
-static uint32_t lora_slot_count(uint64_t rb) { return rb <= 16u ? 16u : 4u; }
-
-// K slices of the adapters' first step, for the second to add up: enough workgroups for two a CU, and at most eight.
+// K slices of the adapters' first step, for the second to add up: at most eight, and two workgroups a CU where a
+// block of 16 rows has four adapters (prompts' have one or two, single tokens' up to 16).
 static uint32_t lora_slices(uint64_t rb, int cus) {
-    const uint64_t per = rb * lora_slot_count(rb), want = (2u * (uint64_t)std::max(1, cus) + per - 1u) / per;
+    const uint64_t want = (2u * (uint64_t)std::max(1, cus) + 4u * rb - 1u) / (4u * rb);
     return (uint32_t)std::max<uint64_t>(1u, std::min<uint64_t>(want, kLoraSlices));
 }
 
@@ -1068,7 +1065,7 @@ static uint32_t lora_slices(uint64_t rb, int cus) {
 // weight (65 .. 1024 rows, 2048 and 8192 rows of K) and cost 3 us at 512 rows of rank 64.
 void lora_shape(LoraParams* p, bool in_product, int cus) {
     const uint32_t rb = (p->rows + 15u) / 16u;
-    p->slots = lora_slot_count(rb);
+    p->slots = rb <= 16u ? 16u : 4u;                         // workgroups that share a row block's distinct adapters
     p->rp32 = (p->rp + kLoraRanks - 1u) / kLoraRanks * kLoraRanks;
     const uint32_t nz = in_product ? 1u : std::max(1u, std::min(lora_slices(rb, cus), (p->k + 511u) / 512u));
     p->uh = in_product ? reinterpret_cast<uint16_t*>(p->u) : nullptr;
@@ -1083,7 +1080,7 @@ uint64_t lora_u_bytes(uint64_t rows, uint32_t rp, int cus) {
     uint64_t b = rows * ((uint64_t)rp + (rp + kLoraRanks - 1u) / kLoraRanks) * sizeof(float);
     for (uint64_t rb = 1; rb <= (rows + 15u) / 16u; ++rb) {
         const uint64_t nz = lora_slices(rb, cus);
-        if (nz == 1u && rb > 16u) break;                     // (and so are all beyond)
+        if (nz == 1u) break;                                 // (and so are all beyond)
         b = std::max(b, nz * std::min(rows, 16u * rb) * rp * sizeof(float));
     }
     return b;
@@ -1102,8 +1099,7 @@ __global__ __launch_bounds__(256, 4) void lora_gemm_prep_kernel(LoraParams p, ui
                                                                 uint2* wq, uint16_t* sc) {
     __shared__ __align__(16) float red[kLoraShrinkLds / 4];
     if (blockIdx.x < nshrink) {
-        const uint32_t n = lora_slots(p), b = blockIdx.x / n;
-        lora_shrink_block(p, blockIdx.x % n, b % p.nz, b / p.nz, red);
+        lora_shrink_block(p, blockIdx.x, red);
     } else {
         pf_gemm_prep_block(blockIdx.x - nshrink, p.x, xh, xl, xe, p.rows, w, scales, p.k, p.n, wq, sc, red);
     }
@@ -1169,7 +1165,7 @@ hipError_t launch_lora_gemm_small(int fmt, const PfSmallParams& q, const LoraPar
 hipError_t launch_lora_expand(const LoraParams& p, const float* part, uint32_t splits, hipStream_t stream) {
     const uint32_t rb = (p.rows + 15u) / 16u;
     if (!lora_ok(p) || p.uh || rb > 65535u || (splits > 1u && !part)) return hipErrorInvalidValue;
-    if ((uint64_t)rb * (p.n / 32u) >= 2048u)
+    if ((uint64_t)rb * (p.n / 32u) >= 1024u)
         hipLaunchKernelGGL((lora_expand_kernel<4>), dim3((p.n + 127u) / 128u, rb), dim3(512), 0, stream, p, part, splits);
     else
         hipLaunchKernelGGL((lora_expand_kernel<1>), dim3(p.n / 32u, rb), dim3(512), 0, stream, p, part, splits);

@@ -125,7 +125,7 @@ struct PfGemmShape {
 };
 PfGemmShape pf_gemm_shape(uint32_t T, uint32_t k, uint32_t n, int cus);
 // p.nt, p.splits, p.kper from pf_gemm_shape; p.part holds splits * T * n floats when splits > 1
-hipError_t launch_pf_gemm(int fmt, const PrefillGemmParams& p, hipStream_t stream);
+hipError_t launch_pf_gemm(int fmt, const PrefillGemmParams& p, hipStream_t stream, bool reduce = true);
 // Prefill GEMM on pre-packed Q4 weights (pf_gemm2_kernel). pack: the packed
 // copy of a Q4 weight [k][n] (k % 32 == 0, n % 128 == 0) into wq (k n / 2
 // bytes) and sc (k n / 16 bytes, the scales times 2^-wf[group]); wf from
@@ -186,10 +186,10 @@ constexpr uint32_t kLoraMaxRows = 16u * 65535u;   // a grid dimension of row blo
 uint64_t lora_u_bytes(uint64_t rows, uint32_t rp, int cus);   // u of calls of up to that many rows
 // Sets nz, kper, slots and u's form (in_product: for launch_lora_gemm2 of one slice) for p's k, rows and u.
 void lora_shape(LoraParams* p, bool in_product, int cus);
-// launch_lora_shrink and the product kernel of launch_pf_gemm_small in one launch, without the sum over
+// The adapters' first step and the product kernel of launch_pf_gemm_small in one launch, without the sum over
 // q.splits slices: launch_lora_expand takes q.part and q.splits and adds them up itself (splits 1: it adds to y)
 hipError_t launch_lora_gemm_small(int fmt, const PfSmallParams& q, const LoraParams& p, hipStream_t stream);
-// launch_pf_gemm_prep and launch_lora_shrink in one launch; launch_pf_gemm2 with the adapters' second step, in
+// launch_pf_gemm_prep (w null: the rows alone) and the first step in one launch; launch_pf_gemm2 with the adapters' second step, in
 // its sums or with those over q.splits
 hipError_t launch_lora_gemm_prep(const LoraParams& p, uint16_t* xh, uint16_t* xl, int32_t* xe, const uint8_t* w,
                                  const uint16_t* scales, uint2* wq, uint16_t* sc, hipStream_t stream);
