@@ -171,7 +171,7 @@ struct PagedItem {
     uint32_t first, state;     // item of the tile's chunk 0, and where its state goes if it is split
     uint32_t row0, n, len;     // the sequence's first row, its rows, keys any of them sees
     int64_t pos0;              // position of its first row
-    bool narrow;
+    uint32_t narrow;
 };
 
 // A sequence's part of the plan.
@@ -212,64 +212,144 @@ __device__ __forceinline__ uint32_t pg_scan(uint32_t v) {
     return v;
 }
 
-// The item of number `item`; false if there is none. All 64 lanes take part,
-// and every wave of the grid gets the same plan.
-__device__ bool paged_item(const PagedAttnParams& p, uint32_t item, PagedItem* it) {
+// What the four waves of a workgroup tell each other of a plan of more than 64 sequences.
+struct PagedPlanLds {
+    float cost[4];
+    uint32_t items[4], split[4];
+    uint32_t ok;
+    PagedItem it;
+};
+
+// The item of number `item`; false if there is none. All threads take part, and every workgroup of the grid gets the
+// same plan. Up to 64 sequences each wave plans by itself, without a barrier. Of more, every wave takes a quarter:
+// its cost, then its items, and the wave whose quarter holds the item looks for it (1024 tokens over 100 positions:
+// 160 us with all of it in every wave, 108 so). MANY: more than 64, in kernels of their own (in one kernel for both the
+// others took 2 us longer: 32 tokens over up to 8192 positions 44 us against 42).
+template <bool MANY>
+__device__ __forceinline__ bool paged_item(const PagedAttnParams& p, uint32_t item, PagedItem* it, PagedPlanLds* lds) {
     const uint32_t lane = threadIdx.x & (kWave - 1);
     const uint32_t seqs = p.g.seqs;
-    const PagedSeqPlan q0 = paged_seq_plan(p, lane);
     auto cost_of = [&](const PagedSeqPlan& q) {
         return (float)q.tiles * (float)q.steps * (q.narrow ? p.narrow_cost : p.wide_cost);
     };
-    float total = wave_sum(cost_of(q0));
-#pragma unroll 4
-    for (uint32_t b = kWave; b < seqs; b += kWave) total += wave_sum(cost_of(paged_seq_plan(p, b + lane)));
-    const float share = fmaxf(total * (float)p.g.KVH / p.target, p.least);
-    uint64_t base = 0, split = 0;                             // items before the sequences b .., those of them that are split
-    PagedSeqPlan next = q0;
-    for (uint32_t b = 0; b < seqs; b += kWave) {
-        const PagedSeqPlan q = next;
-        if (b + kWave < seqs) next = paged_seq_plan(p, b + kWave + lane);   // (on its way while these are looked through)
+    float share = 0.f;
+    auto set_share = [&](float total) { share = fmaxf(total * (float)p.g.KVH / p.target, p.least); };
+    auto chunks_of = [&](const PagedSeqPlan& q, uint32_t* per) {
         const float per_f = ceilf(share / (q.narrow ? p.narrow_cost : p.wide_cost));
-        const uint32_t per = min((uint32_t)fminf(fmaxf(per_f, 1.f), 1e9f), max(q.steps, 1u));
-        const uint32_t chunks = max((q.steps + per - 1u) / per, 1u);
-        // (more than any grid has: such a sequence is left out below, and so is what follows it)
-        const uint32_t mine = (uint32_t)min((uint64_t)p.g.KVH * q.tiles * chunks, (uint64_t)kPgMaxItems);
+        *per = min((uint32_t)fminf(fmaxf(per_f, 1.f), 1e9f), max(q.steps, 1u));
+        return max((q.steps + *per - 1u) / *per, 1u);
+    };
+    // (more than any grid has: such a sequence is left out below, and so is what follows it)
+    auto items_of = [&](const PagedSeqPlan& q, uint32_t chunks) {
+        return (uint32_t)min((uint64_t)p.g.KVH * q.tiles * chunks, (uint64_t)kPgMaxItems);
+    };
+    uint64_t base = 0, split = 0;                             // items before the sequences b .., those of them that are split
+    // looks among sequences b .. b + 63 (lane's plan: q); 0: not there, 1: found, 2: there, but left out
+    auto find = [&](const PagedSeqPlan& q, uint32_t b) {
+        uint32_t per;
+        const uint32_t chunks = chunks_of(q, &per), mine = items_of(q, chunks);
         const uint32_t sum = pg_scan(mine), apart = pg_scan(chunks > 1u ? mine : 0u);
         const uint64_t end = base + sum, begin = end - mine;
         const uint64_t hit = __ballot(item >= begin && item < end);
-        if (hit) {
-            const int w = __builtin_ctzll(hit);
-            auto u = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, w); };
-            const uint64_t e0 = base + u(sum), b0 = e0 - u(mine);
-            // row offsets that are none can ask for more items than the grid has, or states than the workspace: all of
-            // such a sequence is left out
-            const uint64_t s1 = split + u(apart);
-            if (e0 > gridDim.x || (u(chunks) > 1u && s1 > p.states)) return false;
-            it->s = b + (uint32_t)w;
-            it->tiles = u(q.tiles);
-            it->chunks = u(chunks);
-            it->per = u(per);
-            it->row0 = u(q.row0);
-            it->n = u(q.n);
-            it->len = u(q.len);
-            it->pos0 = (int64_t)((uint64_t)u((uint32_t)(uint64_t)q.pos0) | ((uint64_t)u((uint32_t)((uint64_t)q.pos0 >> 32)) << 32));
-            it->narrow = u(q.narrow ? 1u : 0u) != 0u;
-            // KV head fastest (a head's items keep to the same XCDs' L2), then the tiles that share a chunk of keys
-            uint32_t r = item - (uint32_t)b0;
-            it->kvh = r % p.g.KVH;
-            r /= p.g.KVH;
-            it->tile = r % it->tiles;
-            it->chunk = r / it->tiles;
-            it->first = (uint32_t)b0 + it->tile * p.g.KVH + it->kvh;
-            it->state = it->chunks > 1u ? (uint32_t)(s1 - u(mine)) + it->tile * p.g.KVH + it->kvh : 0u;
-            return true;
+        if (!hit) {
+            base += (uint32_t)__builtin_amdgcn_readlane((int)sum, kWave - 1);
+            split += (uint32_t)__builtin_amdgcn_readlane((int)apart, kWave - 1);
+            return 0;
         }
-        base += (uint32_t)__builtin_amdgcn_readlane((int)sum, kWave - 1);
-        split += (uint32_t)__builtin_amdgcn_readlane((int)apart, kWave - 1);
-        if (base > item) return false;
+        const int w = __builtin_ctzll(hit);
+        auto u = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, w); };
+        const uint64_t e0 = base + u(sum), b0 = e0 - u(mine);
+        // row offsets that are none can ask for more items than the grid has, or states than the workspace: all of
+        // such a sequence is left out
+        const uint64_t s1 = split + u(apart);
+        if (e0 > gridDim.x || (u(chunks) > 1u && s1 > p.states)) return 2;
+        it->s = b + (uint32_t)w;
+        it->tiles = u(q.tiles);
+        it->chunks = u(chunks);
+        it->per = u(per);
+        it->row0 = u(q.row0);
+        it->n = u(q.n);
+        it->len = u(q.len);
+        it->pos0 = (int64_t)((uint64_t)u((uint32_t)(uint64_t)q.pos0) | ((uint64_t)u((uint32_t)((uint64_t)q.pos0 >> 32)) << 32));
+        it->narrow = u(q.narrow ? 1u : 0u);
+        // KV head fastest (a head's items keep to the same XCDs' L2), then the tiles that share a chunk of keys
+        uint32_t r = item - (uint32_t)b0;
+        it->kvh = r % p.g.KVH;
+        r /= p.g.KVH;
+        it->tile = r % it->tiles;
+        it->chunk = r / it->tiles;
+        it->first = (uint32_t)b0 + it->tile * p.g.KVH + it->kvh;
+        it->state = it->chunks > 1u ? (uint32_t)(s1 - u(mine)) + it->tile * p.g.KVH + it->kvh : 0u;
+        return 1;
+    };
+    if constexpr (!MANY) {
+        const PagedSeqPlan q = paged_seq_plan(p, lane);
+        set_share(wave_sum(cost_of(q)));
+        return find(q, 0) == 1;
     }
-    return false;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t quarter = ((seqs + 4u * kWave - 1u) / (4u * kWave)) * kWave;
+    const uint32_t s0 = wave * quarter, s1 = min(seqs, s0 + quarter);
+    const PagedSeqPlan q0 = paged_seq_plan(p, s0 + lane);     // (kept: up to 256 sequences are read once)
+    float cost = cost_of(q0);
+#pragma unroll 4
+    for (uint32_t b = s0 + kWave; b < s1; b += kWave) cost += cost_of(paged_seq_plan(p, b + lane));
+    cost = wave_sum(cost);
+    if (lane == 0) lds->cost[wave] = cost;
+    __syncthreads();
+    set_share((lds->cost[0] + lds->cost[1]) + (lds->cost[2] + lds->cost[3]));
+    uint32_t items = 0, apart = 0;                            // (no more than kPgMaxItems a lane: the sums fit 32 bits)
+    auto count = [&](const PagedSeqPlan& q) {
+        uint32_t per;
+        const uint32_t chunks = chunks_of(q, &per), mine = items_of(q, chunks);
+        items = min(items + mine, kPgMaxItems);
+        apart = min(apart + (chunks > 1u ? mine : 0u), kPgMaxItems);
+    };
+    count(q0);
+#pragma unroll 4
+    for (uint32_t b = s0 + kWave; b < s1; b += kWave) count(paged_seq_plan(p, b + lane));
+    items = pg_scan(items);
+    apart = pg_scan(apart);
+    if (lane == kWave - 1) {
+        lds->items[wave] = items;
+        lds->split[wave] = apart;
+    }
+    if (threadIdx.x == 0) lds->ok = 0;
+    __syncthreads();
+    uint64_t before = 0;
+    bool here = false;
+    for (uint32_t w = 0; w < 4; ++w) {
+        const uint32_t n = __builtin_amdgcn_readfirstlane((int)lds->items[w]);
+        if (w == wave && item >= before && item < before + n) here = true;
+        if (w < wave) {
+            base += n;
+            split += (uint32_t)__builtin_amdgcn_readfirstlane((int)lds->split[w]);
+        }
+        before += n;
+    }
+    if (item >= before) return false;
+    if (here) {
+        int found = 0;
+        PagedSeqPlan next = q0;
+        for (uint32_t b = s0; b < s1 && !found; b += kWave) {
+            const PagedSeqPlan q = next;
+            if (b + kWave < s1) next = paged_seq_plan(p, b + kWave + lane);   // (on its way while these are looked through)
+            found = find(q, b);
+        }
+        if (found == 1 && lane == 0) {
+            lds->it = *it;
+            lds->ok = 1;
+        }
+    }
+    __syncthreads();
+    if (!__builtin_amdgcn_readfirstlane((int)lds->ok)) return false;
+    static_assert(sizeof(PagedItem) % 4 == 0, "copied by words");
+    const uint32_t* from = reinterpret_cast<const uint32_t*>(&lds->it);
+    uint32_t words[sizeof(PagedItem) / 4];
+#pragma unroll
+    for (uint32_t i = 0; i < sizeof(PagedItem) / 4; ++i) words[i] = (uint32_t)__builtin_amdgcn_readfirstlane((int)from[i]);
+    *it = __builtin_bit_cast(PagedItem, words);
+    return true;
 }
 
 // Where a key's row starts, in units of 16 bytes from the pool's first byte
@@ -1271,14 +1351,15 @@ __device__ __forceinline__ void paged_wide(const PagedAttnParams& p, const Paged
 
 // WIDE false: every sequence has at most 16 rows a KV head (single tokens), and
 // the kernel is built without the wide items' registers and LDS.
-template <int HD, bool F16, bool WIDE>
+template <int HD, bool F16, bool WIDE, bool MANY>
 __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnParams p) {
     constexpr uint32_t kNarrowLds = (4u * 16u * (HD + 4u) + 128u) * 4u;
     constexpr uint32_t kWideLds = 4u * pg_wide_keys(F16) * HD * 2u + (F16 ? 0u : pg_wide_keys(F16) * 8u);
     __shared__ __align__(256) char smem[WIDE && kWideLds > kNarrowLds ? kWideLds : kNarrowLds];
     __shared__ uint32_t shared;
+    __shared__ PagedPlanLds plan;
     PagedItem it;
-    if (!paged_item(p, blockIdx.x, &it)) return;
+    if (!paged_item<MANY>(p, blockIdx.x, &it, &plan)) return;
     if constexpr (WIDE) {
         if (!it.narrow) {
             paged_wide<HD, F16>(p, it, smem, &shared);

@@ -66,7 +66,11 @@ hipError_t launch_paged_attn(const PagedAttnParams& in, bool f16, int cus, hipSt
     const uint64_t items = paged_attn_items(p.g.rows, p.g.seqs, p.G, p.g.KVH, cus);
     if (items > kPgMaxItems) return hipErrorInvalidValue;
     const dim3 grid((uint32_t)items), block(256);
-#define QORA_PAGED(HD_, F_, W_) hipLaunchKernelGGL((paged_attn_kernel<HD_, F_, W_>), grid, block, 0, stream, p)
+#define QORA_PAGED(HD_, F_, W_)                                                                                     \
+    do {                                                                                                            \
+        if (p.g.seqs > kWave) hipLaunchKernelGGL((paged_attn_kernel<HD_, F_, W_, true>), grid, block, 0, stream, p); \
+        else hipLaunchKernelGGL((paged_attn_kernel<HD_, F_, W_, false>), grid, block, 0, stream, p);                \
+    } while (0)
 #define QORA_PAGED_W(HD_, F_) \
     do {                      \
         if (wide) QORA_PAGED(HD_, F_, true); else QORA_PAGED(HD_, F_, false); \
