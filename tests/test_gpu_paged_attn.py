@@ -377,6 +377,32 @@ def test_row_offsets_that_are_none(ctx, pkg):
         ctx.paged_attn_release(aid)
 
 
+def test_row_offsets_that_are_none_of_many(ctx, pkg):
+    """The same with more sequences than one wave plans, which ask for more items than there are workgroups."""
+    r = rng(25)
+    H, KVH, hd, n = 8, 2, 64, 200
+    batch, pool, q = _inputs(pkg, r, "f16", "head", 16, H, KVH, hd, [(1, 40 + 30 * (i % 7)) for i in range(n)], pad_rows=1)
+    good = batch.row_start.copy()
+    ref, tol = attention64(pool, batch, q, H)
+    at = np.arange(n + 1)
+    with device(ctx) as d:
+        kv, b = pool.put(d), batch.put(pkg, d)
+        dq, out = d.put(q), d.put(np.full(q.shape, 77.0, np.float32))
+        aid = ctx.paged_attn_prepare(batch.rows, n, H, KVH, hd)
+        for starts in (at % 2 * n, n - at, at * 10 ** 6, at - n, np.full(n + 1, -2 ** 31), np.where(at < 150, at, at % 2 * n)):
+            ctx.h2d(batch.d[0], starts.astype(np.int32))
+            ctx.paged_attn_run(aid, kv, b, dq, out)
+            ctx.synchronize()
+            assert np.all(d.get(out, q.shape, np.float32)[n:] == 77.0)      # a row of nobody
+        ctx.h2d(batch.d[0], good)
+        for _ in range(2):
+            ctx.h2d(out, np.full(q.shape, 77.0, np.float32))
+            ctx.paged_attn_run(aid, kv, b, dq, out)
+            ctx.synchronize()
+            _check(d.get(out, q.shape, np.float32), batch, ref, tol)
+        ctx.paged_attn_release(aid)
+
+
 def test_attention_refusals(ctx, pkg):
     r = rng(19)
     H, KVH, hd = 8, 2, 64
