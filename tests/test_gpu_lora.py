@@ -112,6 +112,29 @@ def test_rows_without_an_adapter_are_the_plain_product(ctx, pkg):
     ctx.lora_release(lid)
 
 
+@pytest.mark.parametrize("fmt,k,n,T", [("q4", 2048, 512, 130), ("q4", 2048, 8192, 200), ("q4", 640, 96, 100),
+                                       ("f16", 2048, 512, 130), ("f16", 512, 4096, 90), ("f16", 4096, 4096, 300),
+                                       ("f16", 512, 2080, 30), ("q4", 4096, 256, 9)])
+def test_no_adapter_changes_no_bit(ctx, pkg, fmt, k, n, T):
+    """Every form of the product: rows without an adapter are qora_hip_gemm's, beside rows that have one."""
+    r = rng(k + T)
+    weight, w = _weight(pkg, r, fmt, k, n)
+    ads = _adapters(pkg, r, [16, 40], k, n)
+    x = r.normal(size=(T, k)).astype(np.float32)
+    wid, lid = ctx.upload(weight), ctx.lora_upload(ads, T)
+    with device(ctx) as d:
+        plain = d.empty(T * n * 4)
+        ctx.check(ctx.lib.qora_hip_gemm(ctx.h, wid, d.put(x), plain, T, None))
+        plain = d.get(plain, (T, n), np.float32)
+        for rows in (np.full(T, -1, np.int32), (np.arange(T) % 5 - 3).astype(np.int32)):
+            y = d.get(_run(ctx, d, wid, lid, x, n, rows), (T, n), np.float32)
+            assert np.array_equal(y[rows < 0], plain[rows < 0])
+            ref, tol = _truth(x, w, ads, rows)
+            assert np.all(np.abs(y - ref) <= tol)
+    ctx.lora_release(lid)
+    ctx.check(ctx.lib.qora_hip_release_weight(ctx.h, wid))
+
+
 def test_rows_of_very_different_size(ctx, pkg):
     """A row's own scale: tiny and huge rows side by side, and one that is not finite."""
     r = rng(3)
