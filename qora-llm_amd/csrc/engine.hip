@@ -2336,11 +2336,12 @@ int gemm_call(qora_hip_ctx* c, uint32_t wid, const float* x, float* y, uint64_t 
     if (lora)
         HIP_TRY(c, launch_lora_gemm_prep(*lora, r.xh, r.xl, r.xe, g.wide && q4 ? (const uint8_t*)w->w : nullptr,
                                          (const uint16_t*)w->scales, (uint2*)wq, (uint16_t*)(wq + g.bq), s));
+    else if (g.wide && q4)
+        HIP_TRY(c, launch_pf_gemm_prep(x, T, r.xh, r.xl, r.xe, (const uint8_t*)w->w, (const uint16_t*)w->scales, K, N,
+                                       (uint2*)wq, (uint16_t*)(wq + g.bq), s));
+    else
+        HIP_TRY(c, launch_pf_rows(PF_ROW_SPLIT, r, T, s));
     if (g.wide) {
-        if (lora) {}
-        else if (q4) HIP_TRY(c, launch_pf_gemm_prep(x, T, r.xh, r.xl, r.xe, (const uint8_t*)w->w, (const uint16_t*)w->scales,
-                                               K, N, (uint2*)wq, (uint16_t*)(wq + g.bq), s));
-        else HIP_TRY(c, launch_pf_rows(PF_ROW_SPLIT, r, T, s));
         PfGemm2Params h{};
         h.xh = r.xh;
         h.xl = r.xl;
@@ -2357,7 +2358,6 @@ int gemm_call(qora_hip_ctx* c, uint32_t wid, const float* x, float* y, uint64_t 
         else HIP_TRY(c, launch_pf_gemm2(g.s2.bm, h, s, true, q4 ? PF_W_RAW : PF_W_F16));
         return QORA_HIP_OK;
     }
-    if (!lora) HIP_TRY(c, launch_pf_rows(PF_ROW_SPLIT, r, T, s));
     int8_t* wf = (int8_t*)(base + 2 * g.bx + g.be);
     if (q4)
         HIP_TRY(c, launch_pf_weight_exp((const uint16_t*)w->scales, K, N / 32, wf, (uint32_t*)(base + 2 * g.bx + g.be + g.bf), s));
